@@ -156,6 +156,97 @@ int simp_gpu_softmax_f32(const float* x_dev, float* y_dev, int64_t rows, int64_t
                          int64_t yoff, int64_t row_stride);
 int simp_gpu_silu_f32(const float* x_dev, const float* mul_dev, float* y_dev, int64_t n);
 
+/* ---- attention over prompts, the 8-bit key/value cache, from logits to the next token ---------
+ * No counterpart in the reference as ops: its models hold attention as loops over one sequence (stories110M.sl:110-170,
+ * llama32_1b_int8_tensor.sl:142-215) and its hosts take a plain argmax (generate_stories110M.cpp:73-83).  These calls
+ * serve batches: sequences of different lengths lie one behind the other ("packed"), sequence s being the rows
+ * offsets[s] .. offsets[s + 1] - 1 of an int32 array of n_seqs + 1 offsets on the device (ascending, within the given
+ * total).  Rows of a packed tensor are heads x head_dim elements, a row stride apart (elements; 0: contiguous), heads
+ * contiguous in a row, so q, k and v may be parts of one projection's output.  Elements are `dtype`; sums, softmax
+ * statistics and scales are f32, and outputs are rounded once.  n_heads is a multiple of n_kv_heads; query head h reads
+ * key/value head h / (n_heads / n_kv_heads).  head_dim is 1 .. 128.  Rows behind the last sequence are left as they are.
+ * Outputs may not overlap inputs unless a call says so.
+ * Offsets, lengths or block numbers out of range are found on the device: what they concern is skipped (outputs of a
+ * skipped sequence are left as they are) and simp_gpu_check_device_status() reports SIMP_ERR_ARG. */
+#define SIMP_DTYPE_F32 0
+#define SIMP_DTYPE_F16 1
+#define SIMP_DTYPE_BF16 2
+
+/* Causal attention over prompts: out_i = sum_j softmax_j(scale * q_i . k_j) v_j over the keys j <= i + (nk - nq) of the
+ * same sequence, nq and nk being its query and key rows: with nk > nq the queries are the last nq places of the text
+ * (a prompt that goes on behind rows which kv8_read brought back).  k_offsets_dev NULL: the same as q_offsets_dev.  A
+ * query row that sees no key (nk < nq) gets zeros.  Keys that a row does not see have no influence on it, NaN and
+ * infinities included.  16-bit types with head_dim 64 or 128 whose rows TMA can address (16-byte pointers and strides)
+ * run on the tcgen05 tensor cores, where the softmax weights are rounded to the 16-bit type before they multiply v;
+ * everything else runs in f32 arithmetic.  The group n_heads / n_kv_heads is at most 128. */
+int simp_gpu_attn_prompt(const void* q_dev, const void* k_dev, const void* v_dev, void* out_dev, const int32_t* q_offsets_dev,
+                         const int32_t* k_offsets_dev, int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t n_heads,
+                         int64_t n_kv_heads, int64_t head_dim, int64_t q_stride, int64_t kv_stride, int64_t out_stride,
+                         float scale, int dtype);
+
+/* A cache of keys and values in 8 bits: a pool of blocks of block_tokens tokens (16, 32, 64 or 128), of one layer.
+ *   k [n_blocks, n_kv_heads, block_tokens, pitch] int8, v [n_blocks, n_kv_heads, block_tokens / 16, pitch, 16] int8
+ * (v holds 16 tokens of one element next to each other: the order in which attention multiplies them), pitch = head_dim
+ * rounded up to a multiple of 32, and one f32 scale per block and head, k_scales and v_scales [n_blocks, n_kv_heads]:
+ * a stored value is integer * scale.  k and v are 16-byte aligned.  Token t of sequence s lies in block
+ * block_table[s * table_stride + t / block_tokens] (int32, device), place t % block_tokens.  The caller owns the memory
+ * and the table; nothing has to be cleared. */
+typedef struct simp_kv8_cache {
+  int8_t* k;
+  int8_t* v;
+  float* k_scales;
+  float* v_scales;
+  int64_t n_blocks, block_tokens, n_kv_heads, head_dim;
+} simp_kv8_cache;
+/* Writes the packed rows k, v (row i of sequence s at place starts[s] + i).  A block's scale is max|x| / 127 over the
+ * tokens that it holds, rounded to f32; values are x / scale to the nearest integer, halves to even.  A block that held
+ * tokens already (starts[s] inside it) keeps the larger of its scale and the new one; where that grows, the tokens
+ * before starts[s] are re-quantised from their integers.  A scale below FLT_MIN is 0 and the block's values are 0.
+ * 8 bits hold no NaN and no infinities: NaN is stored as 0, +-infinity as +-127, and neither counts for the scale.
+ * No block may be written for two sequences in one call. */
+int simp_gpu_kv8_append(const simp_kv8_cache* cache, const int32_t* block_table_dev, int64_t table_stride, const void* k_dev,
+                        const void* v_dev, int64_t kv_stride, const int32_t* offsets_dev, const int32_t* starts_dev,
+                        int64_t n_seqs, int64_t total, int dtype);
+/* Reads places starts[s] .. of each sequence back into packed rows k, v (integer * scale, rounded to dtype). */
+int simp_gpu_kv8_read(const simp_kv8_cache* cache, const int32_t* block_table_dev, int64_t table_stride, void* k_dev,
+                      void* v_dev, int64_t kv_stride, const int32_t* offsets_dev, const int32_t* starts_dev, int64_t n_seqs,
+                      int64_t total, int dtype);
+/* Attention of one query token per sequence, q and out [n_seqs, n_heads, head_dim], over the first lengths[s] (int32,
+ * device, 0 .. max_len) places of its cache; max_len is at most table_stride * block_tokens.  A sequence of length 0
+ * gets zeros.  Long caches are split over blocks of the GPU and joined in a fixed order (library scratch: make the first
+ * call of a size before recording it). */
+int simp_gpu_attn_kv8(const simp_kv8_cache* cache, const int32_t* block_table_dev, int64_t table_stride, const void* q_dev,
+                      void* out_dev, int64_t q_stride, int64_t out_stride, const int32_t* lengths_dev, int64_t n_seqs,
+                      int64_t max_len, int64_t n_heads, float scale, int dtype);
+
+/* What stands between logits and the next token, per row r of [rows, vocab].  Every array is optional (NULL).
+ * n(t) = how often token t stands in tokens[token_offsets[r] .. token_offsets[r + 1]) (the row's prompt and output so
+ * far; ids outside 0 .. vocab - 1, such as padding, are ignored).  In this order, in f32, for every token t:
+ *   n > 0:  x = x > 0 ? x / repetition[r] : x * repetition[r];   x = x - (frequency[r] * n + presence[r])
+ *   x = x + bias_values[e] for the LAST entry e of bias_offsets[r] .. with bias_tokens[e] == t
+ *   bit t % 32 of word t / 32 of the row's mask is 0:  x = -infinity
+ * n_tokens and n_bias are the lengths of the id lists; allowed_stride is the distance of the rows' masks in words
+ * (at least ceil(vocab / 32)), 0: one mask for all rows. */
+typedef struct simp_logits_rules {
+  const int32_t* tokens;
+  const int32_t* token_offsets; /* [rows + 1] */
+  int64_t n_tokens;
+  const float* repetition; /* [rows]; positive */
+  const float* frequency;  /* [rows] */
+  const float* presence;   /* [rows] */
+  const int32_t* bias_tokens;
+  const float* bias_values;
+  const int32_t* bias_offsets; /* [rows + 1] */
+  int64_t n_bias;
+  const uint32_t* allowed;
+  int64_t allowed_stride;
+} simp_logits_rules;
+/* out may be the logits themselves.  argmax_dev (int32 [rows], may be NULL) receives the token with the largest result as
+ * it is written (the lowest of equals; NaN is passed over), -1 where nothing is larger than -infinity.  Uses a little
+ * library scratch when argmax_dev is given.  row_stride in elements, 0: vocab. */
+int simp_gpu_logits_process(const void* logits_dev, void* out_dev, int64_t rows, int64_t vocab, int64_t row_stride,
+                            const simp_logits_rules* rules, int32_t* argmax_dev, int dtype);
+
 /* ---- int8 quantise / dequantise ------------------------------------------------------------
  * Scalar model code in the reference, not ops: y = (int8) trunc(clamp(x*scale, -128, 127))
  * (examples/llama2/llama32_1b_int8_tensor.sl:96-103; without the clamp in
@@ -183,7 +274,7 @@ int simp_gpu_event_destroy(void* event);
  * Between record_begin and record_end the calls are recorded, not executed; only the simp_gpu_* compute entry
  * points with device pointers may be called (no alloc / upload / download / sync, no first call of an op
  * family -- run the sequence once before recording it).  Pointers and shapes are frozen into the recording,
- * library scratch included: simp_gpu_matmul_i4 and simp_gpu_conv2d_f32 use it, so a recorded call of those that
+ * library scratch included: simp_gpu_matmul_i4, simp_gpu_conv2d_f32, simp_gpu_attn_kv8 and simp_gpu_logits_process use it, so a recorded call of those that
  * would need MORE scratch than any earlier call fails with SIMP_ERR_STATE (run it once first); scratch that a
  * live recording uses is kept until the recording is destroyed, whatever later calls need.  Destroy every
  * recording before simp_gpu_shutdown. */

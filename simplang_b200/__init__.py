@@ -65,6 +65,11 @@ _SIGNATURES = {
     "simp_gpu_matmul_i4": [vp, vp, vp, i64, i64, i64],
     "simp_gpu_tensor_gather": [vp, vp, vp, i64, i64, i64, i64, i64],
     "simp_gpu_conv2d_f32": [vp, vp, vp, vp] + [i64] * 11,
+    "simp_gpu_attn_prompt": [vp] * 6 + [i64] * 9 + [C.c_float, C.c_int],
+    "simp_gpu_kv8_append": [vp, vp, i64, vp, vp, i64, vp, vp, i64, i64, C.c_int],
+    "simp_gpu_kv8_read": [vp, vp, i64, vp, vp, i64, vp, vp, i64, i64, C.c_int],
+    "simp_gpu_attn_kv8": [vp, vp, i64, vp, vp, i64, i64, vp, i64, i64, i64, C.c_float, C.c_int],
+    "simp_gpu_logits_process": [vp, vp, i64, i64, i64, vp, vp, C.c_int],
     "simp_gpu_record_begin": [],
     "simp_gpu_record_end": [C.POINTER(vp)],
     "simp_gpu_replay": [vp, i64],
@@ -227,6 +232,69 @@ def quantize_i8(x, y, n, scale=127.0, clamp=True):
 
 def dequantize_i32(acc, y, n, divisor=65536.0):
     check(lib().simp_gpu_dequantize_i32(_p(acc), _p(y), n, divisor))
+
+
+# ------------------------------------------------------------------------- batched serving ops (device pointers)
+F32, F16, BF16 = 0, 1, 2   # SIMP_DTYPE_*
+
+
+class Kv8Cache(C.Structure):
+    """simp_kv8_cache: where the blocks of an 8-bit key/value cache lie and how they are shaped."""
+    _fields_ = [(n, vp) for n in ("k", "v", "k_scales", "v_scales")] + \
+               [(n, i64) for n in ("n_blocks", "block_tokens", "n_kv_heads", "head_dim")]
+
+
+class LogitsRules(C.Structure):
+    """simp_logits_rules: what logits_process applies to each row."""
+    _fields_ = [("tokens", vp), ("token_offsets", vp), ("n_tokens", i64), ("repetition", vp), ("frequency", vp), ("presence", vp),
+                ("bias_tokens", vp), ("bias_values", vp), ("bias_offsets", vp), ("n_bias", i64), ("allowed", vp), ("allowed_stride", i64)]
+
+
+def kv8_cache(k, v, k_scales, v_scales, n_blocks, block_tokens, n_kv_heads, head_dim) -> Kv8Cache:
+    """Handle of an 8-bit cache in the caller's memory (device buffers or addresses); it keeps no reference to them."""
+    return Kv8Cache(_p(k), _p(v), _p(k_scales), _p(v_scales), n_blocks, block_tokens, n_kv_heads, head_dim)
+
+
+def kv8_bytes(n_blocks, block_tokens, n_kv_heads, head_dim):
+    """(bytes of k, bytes of v, bytes of k_scales, bytes of v_scales) that a cache of this shape takes."""
+    data = n_blocks * n_kv_heads * block_tokens * ((head_dim + 31) // 32 * 32)
+    return data, data, 4 * n_blocks * n_kv_heads, 4 * n_blocks * n_kv_heads
+
+
+def logits_rules(tokens=None, token_offsets=None, n_tokens=0, repetition=None, frequency=None, presence=None, bias_tokens=None,
+                 bias_values=None, bias_offsets=None, n_bias=0, allowed=None, allowed_stride=0) -> LogitsRules:
+    """Rules from device buffers or addresses; like every handle here it keeps no reference to them."""
+    return LogitsRules(_p(tokens), _p(token_offsets), n_tokens, _p(repetition), _p(frequency), _p(presence), _p(bias_tokens),
+                       _p(bias_values), _p(bias_offsets), n_bias, _p(allowed), allowed_stride)
+
+
+def attn_prompt(q, k, v, out, q_offsets, k_offsets, n_seqs, total_q, total_k, n_heads, n_kv_heads, head_dim, q_stride=0, kv_stride=0,
+                out_stride=0, scale=None, dtype=F32):
+    """Causal attention over packed prompts; scale defaults to 1 / sqrt(head_dim)."""
+    scale = max(head_dim, 1) ** -0.5 if scale is None else scale
+    check(lib().simp_gpu_attn_prompt(_p(q), _p(k), _p(v), _p(out), _p(q_offsets), _p(k_offsets), n_seqs, total_q, total_k, n_heads,
+                                     n_kv_heads, head_dim, q_stride, kv_stride, out_stride, scale, dtype))
+
+
+def kv8_append(cache, block_table, table_stride, k, v, offsets, starts, n_seqs, total, kv_stride=0, dtype=F32):
+    check(lib().simp_gpu_kv8_append(C.byref(cache), _p(block_table), table_stride, _p(k), _p(v), kv_stride, _p(offsets), _p(starts),
+                                    n_seqs, total, dtype))
+
+
+def kv8_read(cache, block_table, table_stride, k, v, offsets, starts, n_seqs, total, kv_stride=0, dtype=F32):
+    check(lib().simp_gpu_kv8_read(C.byref(cache), _p(block_table), table_stride, _p(k), _p(v), kv_stride, _p(offsets), _p(starts),
+                                  n_seqs, total, dtype))
+
+
+def attn_kv8(cache, block_table, table_stride, q, out, lengths, n_seqs, max_len, n_heads, q_stride=0, out_stride=0, scale=None, dtype=F32):
+    """Attention of one query token per sequence over an 8-bit cache; scale defaults to 1 / sqrt(head_dim)."""
+    scale = max(cache.head_dim, 1) ** -0.5 if scale is None else scale
+    check(lib().simp_gpu_attn_kv8(C.byref(cache), _p(block_table), table_stride, _p(q), _p(out), q_stride, out_stride, _p(lengths),
+                                  n_seqs, max_len, n_heads, scale, dtype))
+
+
+def logits_process(logits, out, rows, vocab, rules, argmax=None, row_stride=0, dtype=F32):
+    check(lib().simp_gpu_logits_process(_p(logits), _p(out), rows, vocab, row_stride, C.byref(rules), _p(argmax), dtype))
 
 
 # ------------------------------------------------------------------------- numpy round trips (tests)

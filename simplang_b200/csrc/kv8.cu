@@ -1,0 +1,633 @@
+// kv8.cu -- the 8-bit key/value cache: writing rows into it, reading them back, attention of single tokens over it.
+//
+// A block holds `bt` tokens of one layer; per block and head one f32 scale.  K lies [token][pitch] (a score contracts
+// over elements), V lies [token / 16][pitch][16 tokens] (an output contracts over tokens), so both are read as they are
+// multiplied: as the s8 operand of warp-level integer MMAs, without a conversion or a transpose on the way.
+#include <algorithm>
+#include <cfloat>
+#include <climits>
+
+#include "llm_ops.cuh"
+
+namespace simp {
+
+struct Kv8View {
+  int8_t* k;
+  int8_t* v;
+  float* ks;
+  float* vs;
+  const int32_t* table;
+  int64_t table_stride;
+  int n_blocks, bt, G, D, pitch;
+};
+
+// ------------------------------------------------------------------------------------------------ write
+// max|x| / 127, IEEE division; a subnormal step could not be divided by and stands for zeros.
+__device__ __forceinline__ float kv8_step(float top) {
+  const float s = __fdiv_rn(top, 127.0f);
+  return s < FLT_MIN ? 0.0f : s;
+}
+__device__ __forceinline__ float kv8_magnitude(float x) {
+  const float a = fabsf(x);
+  return a <= FLT_MAX ? a : 0.0f;   // NaN and infinities do not count
+}
+// x / s to the nearest integer, halves to even, exactly: the product with 1 / s is within one of it, and the remainder
+// x - n s has no rounding error (n <= 127, |x - n s| < 2 s: a multiple of the smaller ulp that fits 24 bits), so it
+// tells which side of a half x lies on.  A plain division would round quotients next to a half onto it.
+__device__ __forceinline__ int kv8_quantise(float x, float s, float inv) {
+  if (s == 0.0f || x != x) return 0;
+  if (fabsf(x) > FLT_MAX) return x > 0.0f ? 127 : -127;
+  float n = rintf(x * inv);
+  const float r2 = 2.0f * fmaf(-n, s, x);
+  if (r2 > s) n += 1.0f;
+  else if (r2 < -s) n -= 1.0f;
+  else if (fabsf(r2) == s && (int(n) & 1)) n += r2 > 0.0f ? 1.0f : -1.0f;
+  return int(fminf(fmaxf(n, -127.0f), 127.0f));
+}
+// A held integer to a larger step: q * old is exact in 64 bits, and a quotient that is not a half differs from it by far
+// more than 64-bit rounding.
+__device__ __forceinline__ int kv8_requantise(int q, double old, double now) {
+  return now > 0.0 ? int(fmin(fmax(rint(double(q) * old / now), -127.0), 127.0)) : 0;
+}
+
+// The part of sequence s that lies in one block: unit = (sequence, block), found by find_unit.
+struct Kv8Span {
+  int seq, row0, a, b;   // packed row of place a of the block; places [a, b) are new
+  int block;
+};
+__device__ __forceinline__ bool kv8_span(const Kv8View& c, int64_t unit, const int32_t* off, const int32_t* starts, int n_seqs,
+                                         int64_t total, int* status, Kv8Span& sp) {
+  const int64_t cap = c.table_stride * c.bt;
+  auto count = [&](int s) {
+    int q0, q1;
+    if (!seq_range(off, s, total, status, q0, q1) || q0 == q1) return 0;
+    const int64_t st = __ldg(starts + s), n = q1 - q0;
+    if (st < 0 || st + n > cap) {
+      report_status(status, STATUS_BAD_RANGE, s);
+      return 0;
+    }
+    return int((st + n - 1) / c.bt - st / c.bt) + 1;
+  };
+  int place;
+  if (!find_unit(unit, n_seqs, count, sp.seq, place)) return false;
+  const int q0 = __ldg(off + sp.seq), n = __ldg(off + sp.seq + 1) - q0, st = __ldg(starts + sp.seq);
+  const int64_t bi = st / c.bt + place, p0 = bi * c.bt;
+  sp.a = int(max(int64_t(st) - p0, int64_t(0)));
+  sp.b = int(min(int64_t(st) + n - p0, int64_t(c.bt)));
+  sp.row0 = int(q0 + (p0 + sp.a - st));
+  sp.block = __ldg(c.table + sp.seq * c.table_stride + bi);
+  if (sp.block < 0 || sp.block >= c.n_blocks) {
+    if (threadIdx.x == 0) report_status(status, STATUS_BAD_BLOCK, sp.block);
+    return false;
+  }
+  return true;
+}
+
+constexpr int KV8_THREADS = 128;
+// One block of 128 threads per (sequence, cache block, head).
+template <typename T>
+__global__ void __launch_bounds__(KV8_THREADS) kv8_append_kernel(Kv8View c, const T* __restrict__ k, const T* __restrict__ v,
+                                                                 int64_t row_stride, const int32_t* __restrict__ off,
+                                                                 const int32_t* __restrict__ starts, int n_seqs, int64_t total,
+                                                                 int* status) {
+  __shared__ float red[33];
+  Kv8Span sp;
+  if (!kv8_span(c, blockIdx.x, off, starts, n_seqs, total, status, sp)) return;
+  const int h = blockIdx.y, n_new = sp.b - sp.a;
+  const T* kr = k + int64_t(sp.row0) * row_stride + int64_t(h) * c.D;
+  const T* vr = v + int64_t(sp.row0) * row_stride + int64_t(h) * c.D;
+  const int64_t sc = int64_t(sp.block) * c.G + h;
+  float topk = 0.0f, topv = 0.0f;
+  for (int i = threadIdx.x; i < n_new * c.D; i += KV8_THREADS) {
+    const int r = i / c.D, d = i - r * c.D;
+    topk = fmaxf(topk, kv8_magnitude(to_f32(kr[r * row_stride + d])));
+    topv = fmaxf(topv, kv8_magnitude(to_f32(vr[r * row_stride + d])));
+  }
+  const float old_k = sp.a ? c.ks[sc] : 0.0f, old_v = sp.a ? c.vs[sc] : 0.0f;
+  topk = block_max(topk, red);
+  topv = block_max(topv, red);
+  const float sk = fmaxf(kv8_step(topk), old_k), sv = fmaxf(kv8_step(topv), old_v);
+  const float ik = sk > 0.0f ? 1.0f / sk : 0.0f, iv = sv > 0.0f ? 1.0f / sv : 0.0f;
+  int8_t* kb = c.k + sc * c.bt * c.pitch;
+  int8_t* vb = c.v + sc * c.bt * c.pitch;
+  if (sp.a && sk != old_k)
+    for (int i = threadIdx.x; i < sp.a * c.pitch; i += KV8_THREADS) kb[i] = int8_t(kv8_requantise(kb[i], old_k, sk));
+  for (int i = threadIdx.x; i < n_new * c.pitch; i += KV8_THREADS) {
+    const int r = i / c.pitch, d = i - r * c.pitch;
+    kb[(sp.a + r) * c.pitch + d] = d < c.D ? int8_t(kv8_quantise(to_f32(kr[r * row_stride + d]), sk, ik)) : int8_t(0);
+  }
+  const bool grew = sp.a && sv != old_v;
+  const int g0 = grew ? 0 : sp.a >> 4, g1 = (sp.b + 15) >> 4;
+  for (int i = threadIdx.x; i < (g1 - g0) * c.pitch; i += KV8_THREADS) {
+    const int g = g0 + i / c.pitch, d = i % c.pitch;
+    int8_t* p = vb + (int64_t(g) * c.pitch + d) * 16;
+    for (int j = 0; j < 16; ++j) {
+      const int t = 16 * g + j;
+      if (t < sp.a) {
+        if (grew) p[j] = int8_t(kv8_requantise(p[j], old_v, sv));
+      } else if (t < sp.b) {
+        p[j] = d < c.D ? int8_t(kv8_quantise(to_f32(vr[(t - sp.a) * row_stride + d]), sv, iv)) : int8_t(0);
+      }
+    }
+  }
+  if (threadIdx.x == 0) {
+    c.ks[sc] = sk;
+    c.vs[sc] = sv;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ read
+template <typename T>
+__global__ void __launch_bounds__(KV8_THREADS) kv8_read_kernel(Kv8View c, T* __restrict__ k, T* __restrict__ v, int64_t row_stride,
+                                                               const int32_t* __restrict__ off, const int32_t* __restrict__ starts,
+                                                               int n_seqs, int64_t total, int* status) {
+  Kv8Span sp;
+  if (!kv8_span(c, blockIdx.x, off, starts, n_seqs, total, status, sp)) return;
+  const int h = blockIdx.y, n = sp.b - sp.a;
+  const int64_t sc = int64_t(sp.block) * c.G + h;
+  const float sk = c.ks[sc], sv = c.vs[sc];
+  const int8_t* kb = c.k + sc * c.bt * c.pitch;
+  const int8_t* vb = c.v + sc * c.bt * c.pitch;
+  T* kr = k + int64_t(sp.row0) * row_stride + int64_t(h) * c.D;
+  T* vr = v + int64_t(sp.row0) * row_stride + int64_t(h) * c.D;
+  for (int i = threadIdx.x; i < n * c.D; i += KV8_THREADS) {
+    const int r = i / c.D, d = i - r * c.D, t = sp.a + r;
+    kr[r * row_stride + d] = from_f32<T>(float(kb[t * c.pitch + d]) * sk);
+    vr[r * row_stride + d] = from_f32<T>(float(vb[(int64_t(t >> 4) * c.pitch + d) * 16 + (t & 15)]) * sv);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ attention
+// out = softmax(scale q . K) V for one token per sequence.  Bound by the cache's bytes, so they go from global memory
+// into the MMA operand registers as they are: mma.m16n8k32 with A = 16 tokens x 32 elements of K (s8) and B = the query,
+// then A = 16 elements x 32 tokens of V (s8) and B = the softmax weights.  Queries and weights become integers of PLANES
+// bytes (16 bits for 16-bit queries, 24 for f32: below the rounding of their own type), one byte plane per B column, so
+// the heads of a group fill the eight columns (4 heads x 2 planes; the third planes of eight heads share one more) and
+// the cache is read once for the whole group.  Integer products are exact; what is rounded is the query (relative to its
+// largest element), the weights (relative to the largest of their 32 tokens) and f32 sums of at most a tile each.
+//
+// A warp owns tiles of 32 tokens.  MMA row <-> token is free to choose: lane (g = lane / 4, t = lane % 4) gets the scores
+// of tokens 4g .. 4g+3 for head t, so softmax maxima are three shuffles, and the weights of a lane pack into one word per
+// plane, which is what the second MMA's B operand wants after one more shuffle: nothing passes through shared memory.
+// Scales multiply scores and weights, never the integers, so blocks of any size (16 and up) may meet in a tile.
+struct AttnKv8Args {
+  Kv8View c;
+  const void* q;
+  void* out;
+  int64_t q_stride, out_stride;
+  const int32_t* lengths;
+  float* part;        // [seq][kv head][group][chunk] x (heads x (D + 2))
+  int* count;         // [seq][kv head][group]
+  int* status;
+  float scale_log2;   // scale * log2(e)
+  int rep, max_len, chunk, max_chunks, dtype;
+};
+
+constexpr int AK_WARPS = 4;
+
+__device__ __forceinline__ void mma_s8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint2 ld_stream_u2(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+// byte `b` of four integers as one word
+template <int B> __device__ __forceinline__ uint32_t bytes_of(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
+  constexpr uint32_t sel = B | ((4 + B) << 4);
+  return __byte_perm(__byte_perm(x0, x1, sel), __byte_perm(x2, x3, sel), 0x5410);
+}
+
+// S = pitch / 32; PLANES = 2 (16-bit queries) or 3 (f32); NH = groups of four heads (1 or 2)
+template <int S, int PLANES, int NH>
+__global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Args a) {
+  constexpr int P = 32 * S, HEADS = 4 * NH, NT = NH + (PLANES == 3 ? 1 : 0);
+  constexpr float QMAX = PLANES == 3 ? 8323072.0f : 32512.0f;      // 127 << 16, 127 << 8: top byte never overflows
+  constexpr float PMAX = PLANES == 3 ? 16777215.0f : 65535.0f;
+  __shared__ __align__(16) int8_t qb[NT * 8][P];                   // byte planes, one row per B column
+  __shared__ float qs[HEADS];
+  __shared__ float om[AK_WARPS][HEADS], ol[AK_WARPS][HEADS];
+  __shared__ __align__(16) float oacc[AK_WARPS][HEADS][P];
+  __shared__ int last;
+  const Kv8View& c = a.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n_groups = (a.rep + HEADS - 1) / HEADS;
+  const int s = blockIdx.z, kvh = blockIdx.y / n_groups, hg = blockIdx.y % n_groups, chunk = blockIdx.x;
+  const int h0 = kvh * a.rep + hg * HEADS, nh = min(HEADS, a.rep - hg * HEADS);
+  const int64_t orow = s * a.out_stride + int64_t(h0) * c.D;
+  const int len = __ldg(a.lengths + s);
+  if (len < 0 || len > a.max_len) {
+    if (threadIdx.x == 0) report_status(a.status, STATUS_BAD_RANGE, s);
+    return;
+  }
+  const int n_chunks = (len + a.chunk - 1) / a.chunk;
+  if (chunk >= n_chunks) {
+    if (len == 0 && chunk == 0)
+      for (int i = threadIdx.x; i < nh * c.D; i += blockDim.x) store_any(a.out, orow + i, 0.0f, a.dtype);
+    return;
+  }
+  // ---- the query as byte planes
+  for (int h = warp; h < HEADS; h += AK_WARPS) {
+    float x[S], top = 0.0f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const int d = lane + 32 * i;
+      x[i] = h < nh && d < c.D ? load_any(a.q, s * a.q_stride + int64_t(h0 + h) * c.D + d, a.dtype) : 0.0f;
+      top = fmaxf(top, fabsf(x[i]));
+      odd = odd || !(fabsf(x[i]) <= FLT_MAX);
+    }
+    top = warp_max(top);
+    odd = __any_sync(0xffffffffu, odd);
+    if (odd) top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      int n = top > 0.0f ? __float2int_rn(__fdiv_rn(x[i], top) * QMAX) : 0;
+      const int lo = int(int8_t(n & 0xff));
+      const int col = (h >> 2) * 8 + 2 * (h & 3), d = lane + 32 * i;
+      if (PLANES == 3) {
+        qb[NH * 8 + 2 * (h & 3) + (h >> 2)][d] = int8_t(lo);
+        n = (n - lo) >> 8;
+        const int mid = int(int8_t(n & 0xff));
+        qb[col + 1][d] = int8_t(mid);
+        qb[col][d] = int8_t((n - mid) >> 8);
+      } else {
+        qb[col + 1][d] = int8_t(lo);
+        qb[col][d] = int8_t((n - lo) >> 8);
+      }
+    }
+    if (PLANES == 3 && NH == 1)
+      for (int i = 0; i < S; ++i) qb[8 + 2 * h + 1][lane + 32 * i] = 0;
+    // a query that is not finite makes its head's result NaN
+    if (lane == 0) qs[h] = odd ? __int_as_float(0x7fc00000) : top / QMAX * a.scale_log2;
+  }
+  __syncthreads();
+  // B fragments: column g, elements 32 i + 8 t .. + 7 (the contraction order of the K loads below)
+  uint32_t qf[NT][S][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      // S even: a 16-byte load covers two steps of a 64-element half; S odd: the last 32 elements by 8-byte loads
+      const int e = (i < (S & ~1)) ? 64 * (i >> 1) + 16 * t + 8 * (i & 1) : 32 * i + 8 * t;
+      const uint2 w = *reinterpret_cast<const uint2*>(&qb[n * 8 + g][e]);
+      qf[n][i][0] = w.x;
+      qf[n][i][1] = w.y;
+    }
+  float hs[NH];   // this lane's heads: 4 n + t
+#pragma unroll
+  for (int n = 0; n < NH; ++n) hs[n] = qs[4 * n + t];
+
+  float m[NH], l[NH], o[2 * S][NT][4];
+#pragma unroll
+  for (int n = 0; n < NH; ++n) m[n] = -INFINITY, l[n] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 2 * S; ++i)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[i][n][r] = 0.0f;
+
+  const int c0 = chunk * a.chunk, c1 = min(len, c0 + a.chunk);
+  const int32_t* table = a.c.table + s * c.table_stride;
+  const int bt_shift = 31 - __clz(c.bt);
+  const int64_t head_bytes = int64_t(c.bt) * P;
+  // block of the 16 tokens from `tok` on; tokens behind the sequence use the block of the tile's first token
+  auto entry = [&](int tile, int half) {
+    const int tok = tile + 16 * half;
+    return __ldg(table + ((tok < len ? tok : tile) >> bt_shift));
+  };
+  for (int tile = c0 + 32 * warp; tile < c1; tile += 32 * AK_WARPS) {
+    int be = entry(tile, g >> 2), bv = entry(tile, t >> 1);
+    const bool bad = be < 0 || be >= c.n_blocks;
+    if (bad) report_status(a.status, STATUS_BAD_BLOCK, be), be = 0;
+    if (bv < 0 || bv >= c.n_blocks) bv = 0;
+    const float ks = __ldg(c.ks + int64_t(be) * c.G + kvh), vs = bad ? 0.0f : __ldg(c.vs + int64_t(be) * c.G + kvh);
+    const int8_t* kp = c.k + (int64_t(be) * c.G + kvh) * head_bytes + (((tile + 4 * g) & (c.bt - 1))) * P;
+    const int8_t* vp = c.v + (int64_t(bv) * c.G + kvh) * head_bytes + int64_t(((tile + 8 * t) & (c.bt - 1)) >> 4) * P * 16 + 8 * (t & 1);
+    uint32_t kw[4][2 * S];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int i = 0; i < S / 2; ++i) {
+        const uint4 w = ld_stream_u4(kp + r * P + 64 * i + 16 * t);
+        kw[r][4 * i] = w.x; kw[r][4 * i + 1] = w.y; kw[r][4 * i + 2] = w.z; kw[r][4 * i + 3] = w.w;
+      }
+      if (S & 1) {
+        const uint2 w = ld_stream_u2(kp + r * P + 32 * (S - 1) + 8 * t);
+        kw[r][2 * S - 2] = w.x; kw[r][2 * S - 1] = w.y;
+      }
+    }
+    uint2 vw[2 * S][2];
+#pragma unroll
+    for (int i = 0; i < 2 * S; ++i) {
+      vw[i][0] = ld_stream_u2(vp + (16 * i + g) * 16);
+      vw[i][1] = ld_stream_u2(vp + (16 * i + 8 + g) * 16);
+    }
+    // ---- scores
+    int acc[2][NT][4];
+#pragma unroll
+    for (int mg = 0; mg < 2; ++mg)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[mg][n][r] = 0;
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+          mma_s8s8(acc[mg][n], kw[2 * mg][2 * i], kw[2 * mg + 1][2 * i], kw[2 * mg][2 * i + 1], kw[2 * mg + 1][2 * i + 1], qf[n][i][0], qf[n][i][1]);
+      }
+    const float vs_top = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 16));
+    const float vs_rel = vs_top > 0.0f ? vs / vs_top : 0.0f;
+    uint32_t pw[NH][PLANES];
+    float fac[NH];
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      float sc[4], tm = -INFINITY;
+      const float f = hs[n] * ks;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int* x = acc[j >> 1][n] + 2 * (j & 1);
+        float v = float(x[0] * 256 + x[1]);
+        if (PLANES == 3) v = fmaf(v, 256.0f, float(acc[j >> 1][NT - 1][2 * (j & 1) + n]));
+        sc[j] = tile + 4 * g + j < len && !bad ? v * f : -INFINITY;
+        tm = fmaxf(tm, sc[j]);
+      }
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, x));
+      const float mn = fmaxf(m[n], tm);
+      const float alpha = m[n] == -INFINITY ? 0.0f : exp2f(m[n] - mn), beta = tm == -INFINITY ? 0.0f : exp2f(tm - mn);
+      float p[4], sum = 0.0f;
+      uint32_t pi[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[j] = sc[j] == -INFINITY ? 0.0f : exp2f(sc[j] - tm);
+        sum += p[j];
+        pi[j] = __float2uint_rn(p[j] * vs_rel * PMAX);
+      }
+      if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+        l[n] *= alpha;
+#pragma unroll
+        for (int i = 0; i < 2 * S; ++i) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[i][n][r] *= alpha;
+          if (PLANES == 3) {
+            o[i][NT - 1][n] *= alpha;
+            o[i][NT - 1][2 + n] *= alpha;
+          }
+        }
+      }
+      l[n] = fmaf(sum, beta, l[n]);
+      m[n] = mn;
+      fac[n] = beta * vs_top;
+      if (PLANES == 3) {
+        pw[n][0] = bytes_of<2>(pi[0], pi[1], pi[2], pi[3]);
+        pw[n][1] = bytes_of<1>(pi[0], pi[1], pi[2], pi[3]);
+        pw[n][PLANES - 1] = bytes_of<0>(pi[0], pi[1], pi[2], pi[3]);
+      } else {
+        pw[n][0] = bytes_of<1>(pi[0], pi[1], pi[2], pi[3]);
+        pw[n][1] = bytes_of<0>(pi[0], pi[1], pi[2], pi[3]);
+      }
+    }
+    // ---- weights to the B operand: column g = (head g / 2, plane g % 2), tokens 8 t .. 8 t + 7
+    uint32_t pf[NT][2];
+    const int src = 8 * t + (g >> 1);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+        const uint32_t hi = __shfl_sync(0xffffffffu, pw[n][0], src + 4 * b), lo = __shfl_sync(0xffffffffu, pw[n][1], src + 4 * b);
+        pf[n][b] = g & 1 ? lo : hi;
+      }
+      if (PLANES == 3) {
+        const uint32_t x = __shfl_sync(0xffffffffu, pw[0][PLANES - 1], src + 4 * b);
+        const uint32_t y = NH == 2 ? __shfl_sync(0xffffffffu, pw[NH - 1][PLANES - 1], src + 4 * b) : 0u;
+        pf[NT - 1][b] = g & 1 ? y : x;
+      }
+    }
+    // ---- values
+#pragma unroll
+    for (int i = 0; i < 2 * S; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        int d[4] = {0, 0, 0, 0};
+        mma_s8u8(d, vw[i][0].x, vw[i][1].x, vw[i][0].y, vw[i][1].y, pf[n][0], pf[n][1]);
+        const bool third = PLANES == 3 && n == NT - 1;
+        const float f0 = third ? fac[0] : fac[n < NH ? n : 0], f1 = third ? fac[NH - 1] : f0;
+        o[i][n][0] = fmaf(float(d[0]), f0, o[i][n][0]);
+        o[i][n][1] = fmaf(float(d[1]), f1, o[i][n][1]);
+        o[i][n][2] = fmaf(float(d[2]), f0, o[i][n][2]);
+        o[i][n][3] = fmaf(float(d[3]), f1, o[i][n][3]);
+      }
+  }
+  // ---- planes together, warps together
+#pragma unroll
+  for (int n = 0; n < NH; ++n) {
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], x);
+    const int h = 4 * n + t;
+    if (g == 0) {
+      om[warp][h] = m[n];
+      ol[warp][h] = l[n];
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * S; ++i)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float v = fmaf(o[i][n][2 * r], 256.0f, o[i][n][2 * r + 1]);
+        if (PLANES == 3) v = fmaf(v, 256.0f, o[i][NT - 1][2 * r + n]);
+        oacc[warp][h][16 * i + 8 * r + g] = v * (1.0f / PMAX);
+      }
+  }
+  __syncthreads();
+  const int stride = HEADS * (c.D + 2);
+  const int64_t slot = (int64_t(s) * gridDim.y + blockIdx.y);
+  float* part = a.part + (slot * a.max_chunks + chunk) * stride;
+  for (int i = threadIdx.x; i < nh * c.D; i += blockDim.x) {
+    const int h = i / c.D, d = i - h * c.D;
+    float top = -INFINITY, den = 0.0f, val = 0.0f;
+#pragma unroll
+    for (int w = 0; w < AK_WARPS; ++w) top = fmaxf(top, om[w][h]);
+#pragma unroll
+    for (int w = 0; w < AK_WARPS; ++w) {
+      const float f = om[w][h] == -INFINITY ? 0.0f : exp2f(om[w][h] - top);
+      den = fmaf(ol[w][h], f, den);
+      val = fmaf(oacc[w][h][d], f, val);
+    }
+    if (n_chunks == 1) {
+      float r = den > 0.0f ? val / den : den;   // den is 0 where every block was out of range; NaN stays
+      if (qs[h] != qs[h]) r = qs[h];
+      store_any(a.out, orow + i, r, a.dtype);
+    } else {
+      part[2 * HEADS + h * c.D + d] = val;
+      if (d == 0) {
+        part[2 * h] = top;
+        part[2 * h + 1] = den;
+      }
+    }
+  }
+  if (n_chunks == 1) return;
+  // ---- the last chunk of this (sequence, head group) to arrive joins all of them, in their order
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(a.count + slot, 1) == n_chunks - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  const float* all = a.part + slot * a.max_chunks * stride;
+  for (int i = threadIdx.x; i < nh * c.D; i += blockDim.x) {
+    const int h = i / c.D, d = i - h * c.D;
+    float top = -INFINITY, den = 0.0f, val = 0.0f;
+    for (int x = 0; x < n_chunks; ++x) top = fmaxf(top, __ldcg(all + int64_t(x) * stride + 2 * h));
+    for (int x = 0; x < n_chunks; ++x) {
+      const float* p = all + int64_t(x) * stride;
+      const float mx = __ldcg(p + 2 * h), f = mx == -INFINITY ? 0.0f : exp2f(mx - top);
+      den = fmaf(__ldcg(p + 2 * h + 1), f, den);
+      val = fmaf(__ldcg(p + 2 * HEADS + h * c.D + d), f, val);
+    }
+    float r = den > 0.0f ? val / den : den;
+    if (qs[h] != qs[h]) r = qs[h];
+    store_any(a.out, orow + i, r, a.dtype);
+  }
+  if (threadIdx.x == 0) a.count[slot] = 0;
+}
+
+template <int S, int PLANES>
+static cudaError_t attn_kv8_launch(int nh, dim3 grid, cudaStream_t st, const AttnKv8Args& a) {
+  if (nh == 1) attn_kv8_kernel<S, PLANES, 1><<<grid, AK_WARPS * 32, 0, st>>>(a);
+  else attn_kv8_kernel<S, PLANES, 2><<<grid, AK_WARPS * 32, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------------------------------------ arguments
+static int kv8_check(const char* who, const simp_kv8_cache* c, const int32_t* table, int64_t table_stride, Kv8View& v) {
+  SIMP_REQUIRE(c, SIMP_ERR_ARG, "%s: cache is null", who);
+  SIMP_REQUIRE(c->head_dim >= 1 && c->head_dim <= 128, SIMP_ERR_SHAPE, "%s: head_dim %lld outside 1 .. 128", who, (long long)c->head_dim);
+  SIMP_REQUIRE(c->block_tokens == 16 || c->block_tokens == 32 || c->block_tokens == 64 || c->block_tokens == 128, SIMP_ERR_SHAPE,
+               "%s: block_tokens %lld is not 16, 32, 64 or 128", who, (long long)c->block_tokens);
+  SIMP_REQUIRE(c->n_blocks >= 1 && c->n_blocks <= INT_MAX && c->n_kv_heads >= 1 && c->n_kv_heads <= 65535, SIMP_ERR_SHAPE,
+               "%s: %lld blocks of %lld heads", who, (long long)c->n_blocks, (long long)c->n_kv_heads);
+  SIMP_REQUIRE(c->k && c->v && c->k_scales && c->v_scales && table, SIMP_ERR_ARG, "%s: null pointer", who);
+  SIMP_REQUIRE(aligned_to(c->k, 16) && aligned_to(c->v, 16), SIMP_ERR_ARG, "%s: the cache's k and v must be 16-byte aligned", who);
+  SIMP_REQUIRE(table_stride >= 1 && table_stride <= INT_MAX / c->block_tokens, SIMP_ERR_SHAPE, "%s: table_stride %lld", who, (long long)table_stride);
+  v = Kv8View{c->k, c->v, c->k_scales, c->v_scales, table, table_stride, int(c->n_blocks), int(c->block_tokens), int(c->n_kv_heads),
+              int(c->head_dim), int((c->head_dim + 31) / 32 * 32)};
+  return SIMP_OK;
+}
+
+static int kv8_rows(const char* who, bool write, const simp_kv8_cache* cache, const int32_t* table, int64_t table_stride, void* k, void* v,
+                    int64_t kv_stride, const int32_t* off, const int32_t* starts, int64_t n_seqs, int64_t total, int dtype) {
+  Kv8View c;
+  SIMP_REQUIRE(dtype_ok(dtype), SIMP_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+  SIMP_REQUIRE(n_seqs >= 0 && total >= 0, SIMP_ERR_ARG, "%s: negative size", who);
+  if (int rc = kv8_check(who, cache, table, table_stride, c)) return rc;
+  if (n_seqs == 0 || total == 0) return SIMP_OK;
+  SIMP_REQUIRE(n_seqs < INT_MAX && total <= INT_MAX, SIMP_ERR_SHAPE, "%s: too many sequences or rows", who);
+  SIMP_REQUIRE(k && v && off && starts, SIMP_ERR_ARG, "%s: null pointer", who);
+  const int64_t row = int64_t(c.G) * c.D;
+  if (kv_stride == 0) kv_stride = row;
+  SIMP_REQUIRE(kv_stride >= row, SIMP_ERR_SHAPE, "%s: kv_stride %lld is shorter than a row", who, (long long)kv_stride);
+  SIMP_REQUIRE(aligned_to(k, dtype_size(dtype)) && aligned_to(v, dtype_size(dtype)), SIMP_ERR_ARG, "%s: misaligned pointer", who);
+  if (int rc = ensure_ready()) return rc;
+  DeviceScope dev;
+  cudaStream_t st = ctx().stream;
+  // a sequence of n rows touches at most (n - 1) / bt + 2 blocks, and never more than n
+  const dim3 grid(unsigned(std::min<int64_t>(total, total / c.bt + 2 * n_seqs)), unsigned(c.G));
+  int* status = ctx().dev_status;
+  auto go = [&](auto zero) {
+    using T = decltype(zero);
+    if (write)
+      kv8_append_kernel<T><<<grid, KV8_THREADS, 0, st>>>(c, static_cast<const T*>(k), static_cast<const T*>(v), kv_stride, off, starts, int(n_seqs), total, status);
+    else
+      kv8_read_kernel<T><<<grid, KV8_THREADS, 0, st>>>(c, static_cast<T*>(k), static_cast<T*>(v), kv_stride, off, starts, int(n_seqs), total, status);
+  };
+  if (dtype == SIMP_DTYPE_F32) go(float());
+  else if (dtype == SIMP_DTYPE_F16) go(__half());
+  else go(__nv_bfloat16());
+  SIMP_LAUNCH_CHECK();
+  return SIMP_OK;
+}
+
+}  // namespace simp
+
+using namespace simp;
+
+SIMP_API int simp_gpu_kv8_append(const simp_kv8_cache* cache, const int32_t* block_table_dev, int64_t table_stride, const void* k_dev,
+                                 const void* v_dev, int64_t kv_stride, const int32_t* offsets_dev, const int32_t* starts_dev,
+                                 int64_t n_seqs, int64_t total, int dtype) {
+  return kv8_rows("kv8_append", true, cache, block_table_dev, table_stride, const_cast<void*>(k_dev), const_cast<void*>(v_dev), kv_stride,
+                  offsets_dev, starts_dev, n_seqs, total, dtype);
+}
+
+SIMP_API int simp_gpu_kv8_read(const simp_kv8_cache* cache, const int32_t* block_table_dev, int64_t table_stride, void* k_dev, void* v_dev,
+                               int64_t kv_stride, const int32_t* offsets_dev, const int32_t* starts_dev, int64_t n_seqs, int64_t total,
+                               int dtype) {
+  return kv8_rows("kv8_read", false, cache, block_table_dev, table_stride, k_dev, v_dev, kv_stride, offsets_dev, starts_dev, n_seqs, total,
+                  dtype);
+}
+
+SIMP_API int simp_gpu_attn_kv8(const simp_kv8_cache* cache, const int32_t* block_table_dev, int64_t table_stride, const void* q_dev,
+                               void* out_dev, int64_t q_stride, int64_t out_stride, const int32_t* lengths_dev, int64_t n_seqs,
+                               int64_t max_len, int64_t n_heads, float scale, int dtype) {
+  AttnKv8Args a{};
+  SIMP_REQUIRE(dtype_ok(dtype), SIMP_ERR_ARG, "attn_kv8: unknown dtype %d", dtype);
+  SIMP_REQUIRE(n_seqs >= 0 && max_len >= 0, SIMP_ERR_ARG, "attn_kv8: negative size");
+  if (int rc = kv8_check("attn_kv8", cache, block_table_dev, table_stride, a.c)) return rc;
+  SIMP_REQUIRE(n_heads >= 1 && n_heads % a.c.G == 0 && n_heads <= 65535, SIMP_ERR_SHAPE, "attn_kv8: %lld query heads over %d key/value heads",
+               (long long)n_heads, a.c.G);
+  SIMP_REQUIRE(max_len <= table_stride * a.c.bt, SIMP_ERR_SHAPE, "attn_kv8: max_len %lld exceeds the table's %lld blocks of %d tokens",
+               (long long)max_len, (long long)table_stride, a.c.bt);
+  if (n_seqs == 0) return SIMP_OK;
+  SIMP_REQUIRE(n_seqs <= 65535, SIMP_ERR_SHAPE, "attn_kv8: more than 65535 sequences");
+  SIMP_REQUIRE(q_dev && out_dev && lengths_dev, SIMP_ERR_ARG, "attn_kv8: null pointer");
+  const int64_t row = n_heads * a.c.D;
+  if (q_stride == 0) q_stride = row;
+  if (out_stride == 0) out_stride = row;
+  SIMP_REQUIRE(q_stride >= row && out_stride >= row, SIMP_ERR_SHAPE, "attn_kv8: a stride is shorter than a row");
+  SIMP_REQUIRE(aligned_to(q_dev, dtype_size(dtype)) && aligned_to(out_dev, dtype_size(dtype)), SIMP_ERR_ARG, "attn_kv8: misaligned pointer");
+  if (int rc = ensure_ready()) return rc;
+  DeviceScope dev;
+  a.q = q_dev;
+  a.out = out_dev;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.lengths = lengths_dev;
+  a.status = ctx().dev_status;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.rep = int(n_heads / a.c.G);
+  a.max_len = int(max_len);
+  a.dtype = dtype;
+  const int nh = a.rep > 4 ? 2 : 1;
+  const int64_t groups = int64_t(a.c.G) * ((a.rep + 4 * nh - 1) / (4 * nh));
+  const int64_t slots = n_seqs * groups;
+  // chunks of at least one tile per warp, so many that the SMs have about three blocks each
+  const int64_t least = 32 * AK_WARPS, want = std::max<int64_t>(1, 3 * int64_t(ctx().sm_count) / slots);
+  a.chunk = int(std::max(least, cdiv(cdiv(std::max<int64_t>(max_len, 1), want), least) * least));
+  a.max_chunks = int(std::max<int64_t>(1, cdiv(max_len, a.chunk)));
+  if (a.max_chunks > 1) {
+    a.part = static_cast<float*>(scratch(size_t(slots) * a.max_chunks * 4 * nh * (a.c.D + 2) * 4, SCRATCH_KV8_PART));
+    if (!a.part) return scratch_failed("attn_kv8");
+    a.count = static_cast<int*>(scratch(size_t(slots) * 4, SCRATCH_KV8_COUNT, true));
+    if (!a.count) return scratch_failed("attn_kv8");
+  }
+  SIMP_REQUIRE(groups <= 65535, SIMP_ERR_SHAPE, "attn_kv8: too many heads");
+  const dim3 grid(unsigned(a.max_chunks), unsigned(groups), unsigned(n_seqs));
+  cudaStream_t st = ctx().stream;
+  const bool wide = dtype == SIMP_DTYPE_F32;
+  cudaError_t e = cudaSuccess;
+  switch (a.c.pitch / 32) {
+    case 1: e = wide ? attn_kv8_launch<1, 3>(nh, grid, st, a) : attn_kv8_launch<1, 2>(nh, grid, st, a); break;
+    case 2: e = wide ? attn_kv8_launch<2, 3>(nh, grid, st, a) : attn_kv8_launch<2, 2>(nh, grid, st, a); break;
+    case 3: e = wide ? attn_kv8_launch<3, 3>(nh, grid, st, a) : attn_kv8_launch<3, 2>(nh, grid, st, a); break;
+    default: e = wide ? attn_kv8_launch<4, 3>(nh, grid, st, a) : attn_kv8_launch<4, 2>(nh, grid, st, a); break;
+  }
+  SIMP_REQUIRE(e == cudaSuccess, SIMP_ERR_CUDA, "attn_kv8 launch failed: %s", cudaGetErrorString(e));
+  return SIMP_OK;
+}

@@ -18,7 +18,7 @@ struct Arena {
   void* p = nullptr;
   size_t cap = 0;
 };
-static Arena g_arena[16];
+static Arena g_arena[24];
 static bool g_capturing = false;          // the library stream is being captured into a recording
 static int g_recordings = 0;              // live recordings (their graphs hold arena pointers)
 static std::vector<void*> g_retired;      // outgrown arena blocks a live recording may still use
@@ -39,7 +39,7 @@ int ensure_ready() {
   return simp_gpu_init(0);
 }
 
-void* scratch(size_t bytes, int slot) {
+void* scratch(size_t bytes, int slot, bool zeroed) {
   std::lock_guard<std::mutex> lk(g_mu);
   Arena& a = g_arena[slot];
   g_scratch_refused = false;
@@ -63,6 +63,11 @@ void* scratch(size_t bytes, int slot) {
     }
     size_t cap = (bytes + (size_t(1) << 20) - 1) & ~((size_t(1) << 20) - 1);
     if (cudaMalloc(&a.p, cap) != cudaSuccess) {
+      a.p = nullptr;
+      return nullptr;
+    }
+    if (zeroed && cudaMemsetAsync(a.p, 0, cap, g_ctx.stream) != cudaSuccess) {
+      cudaFree(a.p);
       a.p = nullptr;
       return nullptr;
     }
@@ -220,6 +225,10 @@ SIMP_API int simp_gpu_check_device_status(void) {
     cudaMemsetAsync(g_ctx.dev_status, 0, 16, g_ctx.stream);
     if (code == 2)   // raised by tensor_gather: an index outside the gathered axis
       return set_error(SIMP_ERR_ARG, "tensor_gather: index %d is outside the gathered axis (row skipped)", where);
+    if (code == 3)   // raised by the kv8 calls
+      return set_error(SIMP_ERR_ARG, "8-bit cache: block number %d is outside the cache (its tokens were skipped)", where);
+    if (code == 4)   // raised by the calls that take offsets or lengths
+      return set_error(SIMP_ERR_ARG, "offsets or lengths of sequence (or row) %d are out of range (skipped)", where);
     return set_error(SIMP_ERR_TIMEOUT, "a bounded device-side wait gave up (code %d, site %d)", code,
                      where);
   }
