@@ -17,4 +17,7 @@ struct AttnPromptArgs {
   int* status;
 };
 
+bool attn_prompt_tc_takes(const AttnPromptArgs& a, int dtype);
+int attn_prompt_tc(const AttnPromptArgs& a, int dtype);
+
 }  // namespace simp
