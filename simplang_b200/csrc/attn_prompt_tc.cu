@@ -1,13 +1,14 @@
 // attn_prompt_tc.cu -- causal attention over packed prompts on the tcgen05 tensor cores: f16 / bf16, head size 64 or 128.
 //
-// One block of 12 warps works on two row tiles ("A" and "B") of one key/value head of one sequence.  A row tile is 128 rows
+// One block of 20 warps works on two row tiles ("A" and "B") of one key/value head of one sequence.  A row tile is 128 rows
 // of the score matrix: 128 / rep consecutive tokens times the rep query heads that share the key/value head (row = token *
 // rep + head), so grouped heads read K and V once, short prompts fill tiles and the causal edge is fine.  Roles:
-//   warps 0-3, 4-7  softmax of tile A, of tile B: one thread per row
-//   warp 8          TMA: Q once, then K and V tiles of 128 keys through a ring of slots
-//   warp 9          issues the MMAs: S = Q K^T (128 x 128, f32 in TMEM), O += P V with P read from TMEM
-//   warp 10         cleans the V tiles at the causal / ragged edge (see below)
-// P (16 bits) overwrites S in place: S_X(j + 1) is issued behind O_X += P_X(j) V(j), and MMAs of one thread run in order.
+//   warps 0-7, 8-15 softmax of tile A, of tile B: two threads per row, 64 keys each, which exchange their maxima
+//   warp 16         TMA: Q once, then K and V tiles of 128 keys through a ring of slots
+//   warps 17, 19    issue the MMAs of tile A, of tile B: S = Q K^T (128 x 128, f32 in TMEM), O += P V with P read from TMEM.
+//                   Issuing blocks while the tensor cores are busy, so one thread for both would leave them idle at its waits
+//   warp 18         cleans the V tiles at the causal / ragged edge (see below)
+// P (16 bits) overwrites S in place: S_X(j + 1) is issued behind O_X += P_X(j) V(j) by the same thread, whose MMAs run in order.
 // While the tensor cores work on one tile, the other tile's softmax runs: 2 x 128 x 128 x D MACs take 4 D cycles per tile and
 // step, its 16384 exponentials 1024, so for D = 128 both are busy about half of the time.
 //
@@ -17,7 +18,7 @@
 //
 // A weight of zero does not hide a NaN or an infinity from an MMA, and a tile may hold keys that some rows must not see:
 // later tokens of the sequence, and rows of the NEXT sequence (or behind the last) where the sequence ends inside the tile.
-// Warp 10 therefore zeroes, in the edge tiles only, V rows behind the sequence and every element that is not finite; a bit
+// Warp 18 therefore zeroes, in the edge tiles only, V rows behind the sequence and every element that is not finite; a bit
 // per such key tells the epilogue to add those elements (read again from global memory) to the rows that do see the key.
 #include <cuda.h>
 #include <algorithm>
@@ -29,16 +30,23 @@
 namespace simp {
 using namespace ptx;
 
-constexpr int TC_THREADS = 384;
+constexpr int TC_THREADS = 640;
+constexpr int W_LOAD = 0, W_MMA = 1, W_EDGE = 3;   // W_MMA: tile A, W_MMA + 1: tile B; 4 .. 19: softmax
 constexpr int TC_EDGE = 4;   // edge tiles of a block: its rows see at most 255 keys more than its first row, so 3
 
+#ifndef TC_EARLY
+#define TC_EARLY (D / 16)
+#endif
 template <int D>
 struct TcShape {
   static constexpr int TILE = 128 * D * 2;              // bytes of 128 rows
   static constexpr int SLOTS = D == 128 ? 5 : 8;
   static constexpr int BARS = 2 * SLOTS + 1 + 6 + TC_EDGE;
-  static constexpr size_t SMEM = 1024 + size_t(2 + SLOTS) * TILE + BARS * 8 + 16 + TC_EDGE * 16;
+  // (1 KB of the 228 belongs to the system: 232448 bytes are a block's most)
+  static constexpr size_t SMEM = size_t(2 + SLOTS) * TILE + BARS * 8 + 16 + TC_EDGE * 16 + 4 * 128 * 4;
 };
+
+static_assert(TcShape<128>::SMEM <= 232448 && TcShape<64>::SMEM <= 232448, "");
 
 struct TcArgs {
   AttnPromptArgs a;
@@ -46,16 +54,17 @@ struct TcArgs {
   uint32_t idesc_s, idesc_o;
 };
 
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// (executed by a whole warp with the same operands; the lane with `leader` issues)
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc, bool leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc)), "r"(uint32_t(leader))
       : "memory");
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc, bool leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc)), "r"(uint32_t(leader))
       : "memory");
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
@@ -63,21 +72,65 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, 
                "r"(bar), "r"(x), "r"(y), "r"(z)
                : "memory");
 }
-__device__ __forceinline__ void tmem_st_32x32(uint32_t t, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t t, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(t)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t t, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-      "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
-      "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(t)
+      "r"(r[14]), "r"(r[15]), "r"(t)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Bounded wait whose usual path is one try: mbar_wait's look at the abort flag first costs a shared-memory round trip.
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int site) {
+  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort_flag, status, site);
+}
+// Barrier of n threads that returns whether `ok` holds for all of them: the warps of a tile give up together, so none is
+// left waiting at the next one.
+__device__ __forceinline__ bool all_of(int id, int n, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbarrier.cta.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(n), "r"(uint32_t(ok))
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// two f32 in a register pair: the packed f32x2 instructions do two operations in one issue slot
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack_f2(float lo, float hi) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float lo_f2(f2 v) { return __uint_as_float(uint32_t(v)); }
+__device__ __forceinline__ float hi_f2(f2 v) { return __uint_as_float(uint32_t(v >> 32)); }
+__device__ __forceinline__ f2 fma_f2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 add_f2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -98,10 +151,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     attn_prompt_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                           const __grid_constant__ CUtensorMap map_v, const TcArgs p) {
   using Sh = TcShape<D>;
-  extern __shared__ uint8_t tc_raw[];
-  const uint32_t base = (smem_u32(tc_raw) + 1023u) & ~1023u;
+  extern __shared__ __align__(1024) uint8_t tc_raw[];   // swizzled tiles start on 1 KB boundaries
+  const uint32_t base = smem_u32(tc_raw);
   const uint32_t q_smem = base, ring = base + 2 * Sh::TILE, bars = ring + Sh::SLOTS * Sh::TILE;
-  uint8_t* generic = tc_raw + (base - smem_u32(tc_raw));
+  uint8_t* generic = tc_raw;
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (Sh::SLOTS + s); };
   const uint32_t q_bar = bars + 8u * (2 * Sh::SLOTS);
@@ -113,18 +166,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8);
   uint32_t* odd_keys = reinterpret_cast<uint32_t*>(tail + 16);   // [TC_EDGE][4]: keys of edge tiles with an element that is not finite
+  float* half_row = reinterpret_cast<float*>(tail + 16 + TC_EDGE * 16);   // [tile][half][row]: what the two threads of a row exchange
   const AttnPromptArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (base & 1023u) {   // never: the declaration asks for it
+    if (threadIdx.x == 0) report_status(a.status, 1, 60);
+    return;
+  }
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < Sh::SLOTS; ++s) {
       mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+      mbar_init(empty_bar(s), 2);
     }
     mbar_init(q_bar, 1);
     for (int x = 0; x < 2; ++x) {
       mbar_init(s_bar(x), 1);
-      mbar_init(p_bar(x), 4);
+      mbar_init(p_bar(x), 9);
       mbar_init(o_bar(x), 1);
     }
     for (int e = 0; e < TC_EDGE; ++e) mbar_init(edge_bar(e), 1);
@@ -158,7 +216,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   const int n = max(n_x[0], n_x[1]);
   const int edge0 = sees(r0) >> 7;                      // tiles from here on hold a key that some row does not see
 
-  if (warp == 9) {
+  if (warp == W_MMA) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
@@ -167,7 +225,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 8) {
+  if (warp == W_LOAD) {
     // ------------------------------------------------------------------ loads
     if (lane == 0 && n > 0) {
       const int tiles = r0 + p.tpt < nq ? 2 : 1;
@@ -179,8 +237,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       bool ok = true;
       for (int i = 0; ok && i < 2 * n; ++i) {
         const int s = i % Sh::SLOTS;
-        if (!mbar_wait(empty_bar(s), ((i / Sh::SLOTS) & 1) ^ 1, abort_flag, a.status, 61)) { ok = false; break; }
-        const bool edge = (i & 1) && (i >> 1) >= edge0;   // lands for warp 10, which passes the slot on
+        if (!wait_bar(empty_bar(s), ((i / Sh::SLOTS) & 1) ^ 1, abort_flag, a.status, 61)) { ok = false; break; }
+        const bool edge = (i & 1) && (i >> 1) >= edge0;   // lands for warp 18, which passes the slot on
         const uint32_t bar = edge ? edge_bar((i >> 1) - edge0) : full_bar(s);
         mbar_arrive_expect_tx(bar, Sh::TILE);
         for (int b = 0; b < D / 64; ++b)
@@ -190,68 +248,97 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);   // let copies in flight land before the block retires
     }
     __syncwarp();
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ MMAs
-    if (lane == 0 && n > 0) {
-      auto wait = [&](uint32_t bar, uint32_t phase, int site) {
-        const bool ok = mbar_wait(bar, phase, abort_flag, a.status, site);
-        tc_fence_after_sync();
-        return ok;
-      };
-      auto wait_slot = [&](int i) { return wait(full_bar(i % Sh::SLOTS), (i / Sh::SLOTS) & 1, 62); };
-      auto scores = [&](int x, int j) {
-        const uint64_t qd = make_smem_desc_sw128(q_smem + x * Sh::TILE, 16u, 1024u);
-        const uint64_t kd = make_smem_desc_sw128(ring + (2 * j % Sh::SLOTS) * Sh::TILE, 16u, 1024u);
+  } else if (warp == W_MMA || warp == W_MMA + 1) {
+    // ------------------------------------------------------------------ MMAs of one tile
+    // The whole warp runs this code with the same values, one lane issues: operands then live in uniform registers.  With a
+    // single lane in the branch each MMA costs a dozen instructions, and the warp shares its scheduler with busy ones.
+    const int x = warp - W_MMA, mine = __shfl_sync(0xffffffffu, n_x[x], 0), other = __shfl_sync(0xffffffffu, n_x[x ^ 1], 0);
+    const int steps = max(mine, other);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const bool leader = lane == 0;
+    auto wait = [&](uint32_t bar, uint32_t phase, int site) {
+      const bool ok = __all_sync(0xffffffffu, wait_bar(bar, phase, abort_flag, a.status, site));
+      tc_fence_after_sync();
+      return ok;
+    };
+    auto commit = [&](uint32_t bar) {
+      if (leader) mma_commit(bar);
+    };
+    const uint32_t s_tmem = tm + 128u * x, o_tmem = tm + 256u + uint32_t(D) * x;
+    const uint64_t qd = make_smem_desc_sw128(q_smem + x * Sh::TILE, 16u, 1024u);
+    const uint64_t ring_k = make_smem_desc_sw128(ring, 16u, 1024u);
+    // V [key][element]: element-major operand, 64-element atoms 16 KB apart, 8 keys 1 KB apart
+    const uint64_t ring_v = make_smem_desc_sw128(ring, 16384u, 1024u);
+    auto scores = [&](int slot, int from, int to) {
+      const uint64_t kd = ring_k + uint64_t(slot * (Sh::TILE / 16));
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {   // 16 elements = 32 bytes; the next 64 elements lie 16 KB further
-          const uint64_t o = uint64_t((s >> 2) * 1024 + (s & 3) * 2);
-          mma_f16_ss(tmem + 128u * x, qd + o, kd + o, p.idesc_s, s > 0);
-        }
-      };
-      auto values = [&](int x, int j) {
-        // V [key][element]: element-major operand, 64-element atoms 16 KB apart, 8 keys 1 KB apart
-        const uint64_t vd = make_smem_desc_sw128(ring + ((2 * j + 1) % Sh::SLOTS) * Sh::TILE, 16384u, 1024u);
+      for (int s = from; s < to; ++s) {   // 16 elements = 32 bytes; the next 64 elements lie 16 KB further
+        const uint64_t o = uint64_t((s >> 2) * 1024 + (s & 3) * 2);
+        mma_f16_ss(s_tmem, qd + o, kd + o, p.idesc_s, s > 0, leader);
+      }
+    };
+    auto values = [&](int slot, bool first) {
+      const uint64_t vd = ring_v + uint64_t(slot * (Sh::TILE / 16));
 #pragma unroll
-        for (int s = 0; s < 8; ++s)          // 16 keys = 8 columns of P, 2 KB of V
-          mma_f16_ts(tmem + 256u + uint32_t(D) * x, tmem + 128u * x + 8u * s, vd + uint64_t(s * 128), p.idesc_o, j > 0 || s > 0);
-      };
-      bool ok = wait(q_bar, 0, 63) && wait_slot(0);
+      for (int s = 0; s < 8; ++s)          // 16 keys = 8 columns of P, 2 KB of V
+        mma_f16_ts(o_tmem, s_tmem + 8u * s, vd + uint64_t(s * 128), p.idesc_o, !(first && s == 0), leader);
+    };
+    bool ok = true;
+    int slot = 0;            // of K(j), then of V(j): slots are taken in the order K(0) V(0) K(1) ...
+    uint32_t phase = 0;
+    auto next = [&] {
+      if (++slot == Sh::SLOTS) slot = 0, phase ^= 1u;
+    };
+    if (mine > 0) {
+      ok = wait(q_bar, 0, 63) && wait(full_bar(0), 0, 62);
       if (ok) {
-        for (int x = 0; x < 2; ++x)
-          if (n_x[x] > 0) {
-            scores(x, 0);
-            mma_commit(s_bar(x));
-          }
-        mma_commit(empty_bar(0));
+        scores(0, 0, D / 16);
+        commit(s_bar(x));
+        commit(empty_bar(0));
+        if (leader && (x == 0 || other == 0)) mbar_arrive(p_bar(x));   // the first turn
       }
-      for (int j = 0; ok && j < n; ++j) {
-        ok = wait_slot(2 * j + 1);
-        if (ok && j + 1 < n) ok = wait_slot(2 * j + 2);
-        for (int x = 0; ok && x < 2; ++x) {
-          if (j >= n_x[x]) continue;
-          ok = wait(p_bar(x), j & 1, 65);
-          if (!ok) break;
-          values(x, j);
-          if (j + 1 < n_x[x]) {
-            scores(x, j + 1);
-            mma_commit(s_bar(x));
-          } else {
-            mma_commit(o_bar(x));
-          }
-        }
+      next();
+      for (int j = 0; ok && j < mine; ++j) {
+        const bool more = j + 1 < mine;
+        const int v_slot = slot;
+        ok = wait(full_bar(v_slot), phase, 62);
+        next();
+        if (ok && more) ok = wait(full_bar(slot), phase, 62);
+        // The weights are there and it is this tile's turn: A B A B ...  Were the tiles' MMAs mixed, both would end late and
+        // both softmaxes run while the tensor cores idle.  The ninth arrival at the barrier is the other tile's thread
+        // passing the turn on, or this one where the other tile has no such step.
+        if (ok) ok = wait(p_bar(x), j & 1, 65);
         if (!ok) break;
-        mma_commit(empty_bar((2 * j + 1) % Sh::SLOTS));
-        if (j + 1 < n) mma_commit(empty_bar((2 * j + 2) % Sh::SLOTS));
+        values(v_slot, j == 0);
+        if (more) scores(slot, 0, TC_EARLY);
+        if (leader) {
+          const int next = x == 0 ? j : j + 1;   // the other tile's step whose turn it is now, if there is one
+          if (next < other) mbar_arrive(p_bar(x ^ 1));
+          else if (more) mbar_arrive(p_bar(x));
+        }
+        if (more) scores(slot, TC_EARLY, D / 16);
+        commit(more ? s_bar(x) : o_bar(x));
+        commit(empty_bar(v_slot));
+        if (more) {
+          commit(empty_bar(slot));
+          next();
+        }
       }
-      if (!ok)
-        for (int i = 0; i < 64; ++i) __nanosleep(1000);
     }
+    // slots that only the other tile works on
+    for (int i = 2 * mine; ok && i < 2 * steps; ++i) {
+      ok = wait(full_bar(slot), phase, 62);
+      if (ok && leader) mbar_arrive(empty_bar(slot));
+      next();
+    }
+    if (!ok)
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
     __syncwarp();
-  } else if (warp == 10) {
+  } else if (warp == W_EDGE) {
     // ------------------------------------------------------------------ V at the edge
     for (int j = edge0; j < n; ++j) {
       const int i = 2 * j + 1;
-      if (!mbar_wait(edge_bar(j - edge0), 0, abort_flag, a.status, 66)) break;
+      if (!wait_bar(edge_bar(j - edge0), 0, abort_flag, a.status, 66)) break;
       uint8_t* v = generic + 2 * Sh::TILE + (i % Sh::SLOTS) * Sh::TILE;
       const int keys = nk - 128 * j;   // rows from here on are not the sequence's
       // (the 128-byte swizzle moves 16-byte pieces inside a row only, so rows are found as if there were none)
@@ -271,39 +358,41 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(full_bar(i % Sh::SLOTS));
     }
-  } else if (warp < 8) {
+  } else {
     // ------------------------------------------------------------------ softmax
-    const int x = warp >> 2, row = threadIdx.x & 127;
+    const int x = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, row = threadIdx.x & 127;
     const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-    const uint32_t s_tmem = tmem + 128u * x + lanes, o_tmem = tmem + 256u + uint32_t(D) * x + lanes;
+    const uint32_t s_tmem = tmem + 128u * x + lanes, o_tmem = tmem + 256u + uint32_t(D) * x + uint32_t(D / 2) * half + lanes;
     const int token = r0 + x * p.tpt + row / a.rep, head = g * a.rep + row % a.rep;
     const bool mine = row < p.tpt * a.rep && token < nq;
     const int lim = mine ? sees(token) : 0;
     const float c = a.scale_log2;
+    volatile float* to = half_row + (2 * x + half) * 128 + row;
+    volatile float* from = half_row + (2 * x + (half ^ 1)) * 128 + row;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int j = 0; j < n_x[x]; ++j) {
-      ok = mbar_wait(s_bar(x), j & 1, abort_flag, a.status, 67);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      ok = wait_bar(s_bar(x), j & 1, abort_flag, a.status, 67);
       tc_fence_after_sync();
-      float s[128];
-#pragma unroll
-      for (int h = 0; h < 4; ++h) tmem_ld_32x32(s_tmem + 32u * h, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * h));
+      uint32_t s[64];
+      tmem_ld_32x32(s_tmem + 64u * half, *reinterpret_cast<uint32_t(*)[32]>(s));
+      tmem_ld_32x32(s_tmem + 64u * half + 32u, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
       tmem_ld_wait();
-      const int see = lim - 128 * j;
-      if (__any_sync(0xffffffffu, see < 128)) {
+      const int see = lim - 128 * j - 64 * half;
+      const bool masked = __any_sync(0xffffffffu, see < 64);
+      if (masked) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i) s[i] = i < see ? s[i] : -INFINITY;
+        for (int i = 0; i < 64; ++i) s[i] = i < see ? s[i] : 0xff800000u;
       }
-      float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+      float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 128; i += 8) {
-        t0 = fmaxf(t0, fmaxf(s[i], s[i + 1]));
-        t1 = fmaxf(t1, fmaxf(s[i + 2], s[i + 3]));
-        t2 = fmaxf(t2, fmaxf(s[i + 4], s[i + 5]));
-        t3 = fmaxf(t3, fmaxf(s[i + 6], s[i + 7]));
-      }
-      const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * c;
+      for (int i = 0; i < 64; i += 2) t[(i >> 1) & 3] = max3(t[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+      float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+      *to = top;
+      // the other half's maximum; behind this point both halves have read S, so P may overwrite it
+      ok = all_of(1 + x, 256, ok);
+      if (!ok) break;
+      top = fmaxf(top, *from) * c;
       if (j == 0) {
         m = top;
       } else if (__any_sync(0xffffffffu, top > m + 8.0f)) {
@@ -311,44 +400,60 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         l *= alpha;
         m = mn;
 #pragma unroll
-        for (int h = 0; h < D / 32; ++h) {
-          uint32_t o[32];
-          tmem_ld_32x32(o_tmem + 32u * h, o);
+        for (int h = 0; h < D / 32; ++h) {   // this half's elements, 16 at a time
+          uint32_t o[16];
+          tmem_ld_32x16(o_tmem + 16u * h, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st_32x32(o_tmem + 32u * h, o);
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st_32x16(o_tmem + 16u * h, o);
         }
       }
       const float off = m == -INFINITY ? 0.0f : m;
-      float sum0 = 0.0f, sum1 = 0.0f;
+      const f2 c2 = pack_f2(c, c), off2 = pack_f2(-off, -off);
+      f2 sum[2] = {0, 0};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t w[32];
+        uint32_t w[16];
+        if (masked) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float e0 = ex2(fmaf(s[64 * h + 2 * i], c, -off)), e1 = ex2(fmaf(s[64 * h + 2 * i + 1], c, -off));
-          sum0 += e0;
-          sum1 += e1;
-          w[i] = pack2<BF16>(e0, e1);
+          for (int i = 0; i < 16; ++i) {
+            const int at = 32 * h + 2 * i;
+            const float y0 = fmaf(__uint_as_float(s[at]), c, -off), y1 = fmaf(__uint_as_float(s[at + 1]), c, -off);
+            const f2 e = pack_f2(at < see ? ex2(y0) : 0.0f, at + 1 < see ? ex2(y1) : 0.0f);
+            sum[i & 1] = add_f2(sum[i & 1], e);
+            w[i] = pack2<BF16>(lo_f2(e), hi_f2(e));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const f2 y = fma_f2(pack_f2(__uint_as_float(s[32 * h + 2 * i]), __uint_as_float(s[32 * h + 2 * i + 1])), c2, off2);
+            const f2 e = pack_f2(ex2(lo_f2(y)), ex2(hi_f2(y)));
+            sum[i & 1] = add_f2(sum[i & 1], e);
+            w[i] = pack2<BF16>(lo_f2(e), hi_f2(e));
+          }
         }
-        tmem_st_32x32(s_tmem + 32u * h, w);
+        tmem_st_32x16(s_tmem + 32u * half + 16u * h, w);
       }
-      l += sum0 + sum1;
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_bar(x));
+      sum[0] = add_f2(sum[0], sum[1]);
+      l += lo_f2(sum[0]) + hi_f2(sum[0]);
     }
-    if (ok && n_x[x] > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_bar(x), 0, abort_flag, a.status, 68));
+    if (ok && n_x[x] > 0) ok = wait_bar(o_bar(x), 0, abort_flag, a.status, 68);
+    *to = l;
+    ok = all_of(1 + x, 256, ok);
     if (ok) {
       tc_fence_after_sync();
+      l += *from;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t(q0 + token) * a.out_stride + int64_t(head) * D) * 2;
+      uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t(q0 + token) * a.out_stride + int64_t(head) * D + (D / 2) * half) * 2;
       uint32_t odd = 0;
       for (int e = 0; e < TC_EDGE * 4; ++e) odd |= odd_keys[e];
 #pragma unroll
-      for (int h = 0; h < D / 32; ++h) {
+      for (int h = 0; h < D / 64; ++h) {
         uint32_t o[32];
         if (n_x[x] > 0) {
           tmem_ld_32x32(o_tmem + 32u * h, o);
@@ -360,7 +465,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           if (odd)   // rare: a key of an edge tile has elements that are not finite
             for (int key = 128 * edge0; key < lim; ++key)
               if ((odd_keys[(key - 128 * edge0) >> 5] >> (key & 31)) & 1u) {
-                const uint16_t* v = static_cast<const uint16_t*>(a.v) + int64_t(k0 + key) * a.kv_stride + int64_t(g) * D + 32 * h;
+                const uint16_t* v = static_cast<const uint16_t*>(a.v) + int64_t(k0 + key) * a.kv_stride + int64_t(g) * D + (D / 2) * half + 32 * h;
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
                   if (odd_halves<BF16>(v[i]) & 0xffffu) {
@@ -384,7 +489,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == W_MMA) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, 512);
   }
