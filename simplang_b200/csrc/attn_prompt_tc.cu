@@ -23,6 +23,7 @@
 #include <cuda.h>
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "attn_prompt.cuh"
 #include "sm100_ptx.cuh"
@@ -34,9 +35,6 @@ constexpr int TC_THREADS = 640;
 constexpr int W_LOAD = 0, W_MMA = 1, W_EDGE = 3;   // W_MMA: tile A, W_MMA + 1: tile B; 4 .. 19: softmax
 constexpr int TC_EDGE = 4;   // edge tiles of a block: its rows see at most 255 keys more than its first row, so 3
 
-#ifndef TC_EARLY
-#define TC_EARLY (D / 16)
-#endif
 template <int D>
 struct TcShape {
   static constexpr int TILE = 128 * D * 2;              // bytes of 128 rows
@@ -85,6 +83,16 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t t, const uint32_t (&r)[16
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
       "r"(r[14]), "r"(r[15]), "r"(t)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t t, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+      "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(t)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -223,7 +231,96 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = *tmem_slot;   // 0: the block allocates every column
+
+  // ------------------------------------------------------------------ MMAs of tile X
+  // The whole warp runs this code with the same values and one lane issues; x, the TMEM columns (all 512 are this block's,
+  // so they start at 0) and the descriptors' bases are constants.  Operands of an MMA then live in uniform registers; from
+  // general ones each costs several more instructions, and the warp shares its scheduler with the softmax of the other
+  // tile, which leaves few slots (beside warps that issue nothing but FFMA an MMA took 113-130 cycles instead of 64).
+  auto mma_role = [&](auto which) {
+    constexpr int x = decltype(which)::value;
+    const int mine = n_x[x], other = n_x[x ^ 1];
+    const int steps = max(mine, other);
+    const bool leader = lane == 0;
+    auto wait = [&](uint32_t bar, uint32_t phase, int site) {
+      const bool ok = __all_sync(0xffffffffu, wait_bar(bar, phase, abort_flag, a.status, site));
+      tc_fence_after_sync();
+      return ok;
+    };
+    auto commit = [&](uint32_t bar) {
+      if (leader) mma_commit(bar);
+    };
+    constexpr uint32_t s_tmem = 128u * x, o_tmem = 256u + uint32_t(D) * x;
+    const uint64_t qd = make_smem_desc_sw128(q_smem + x * Sh::TILE, 16u, 1024u);
+    const uint64_t ring_k = make_smem_desc_sw128(ring, 16u, 1024u);
+    // V [key][element]: element-major operand, 64-element atoms 16 KB apart, 8 keys 1 KB apart
+    const uint64_t ring_v = make_smem_desc_sw128(ring, 16384u, 1024u);
+    auto scores = [&](int slot) {
+      const uint64_t kd = ring_k + uint64_t(slot * (Sh::TILE / 16));
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {   // 16 elements = 32 bytes; the next 64 elements lie 16 KB further
+        const uint64_t o = uint64_t((s >> 2) * 1024 + (s & 3) * 2);
+        mma_f16_ss(s_tmem, qd + o, kd + o, p.idesc_s, s > 0, leader);
+      }
+    };
+    auto values = [&](int slot, bool first) {
+      const uint64_t vd = ring_v + uint64_t(slot * (Sh::TILE / 16));
+#pragma unroll
+      for (int s = 0; s < 8; ++s)          // 16 keys = 8 columns of P, 2 KB of V
+        mma_f16_ts(o_tmem, s_tmem + 8u * s, vd + uint64_t(s * 128), p.idesc_o, !(first && s == 0), leader);
+    };
+    bool ok = true;
+    int slot = 0;            // of K(j), then of V(j): slots are taken in the order K(0) V(0) K(1) ...
+    uint32_t phase = 0;
+    auto next = [&] {
+      if (++slot == Sh::SLOTS) slot = 0, phase ^= 1u;
+    };
+    if (mine > 0) {
+      ok = wait(q_bar, 0, 63) && wait(full_bar(0), 0, 62);
+      if (ok) {
+        scores(0);
+        commit(s_bar(x));
+        commit(empty_bar(0));
+        if (leader && (x == 0 || other == 0)) mbar_arrive(p_bar(x));   // the first turn
+      }
+      next();
+      for (int j = 0; ok && j < mine; ++j) {
+        const bool more = j + 1 < mine;
+        const int v_slot = slot;
+        ok = wait(full_bar(v_slot), phase, 62);
+        next();
+        if (ok && more) ok = wait(full_bar(slot), phase, 62);
+        // The weights are there and it is this tile's turn: A B A B ...  Were the tiles' MMAs mixed, both would end late and
+        // both softmaxes run while the tensor cores idle.  The ninth arrival at the barrier is the other tile's thread
+        // passing the turn on, or this one where the other tile has no such step.
+        if (ok) ok = wait(p_bar(x), j & 1, 65);
+        if (!ok) break;
+        values(v_slot, j == 0);
+        if (more) scores(slot);
+        if (leader) {
+          const int next = x == 0 ? j : j + 1;   // the other tile's step whose turn it is now, if there is one
+          if (next < other) mbar_arrive(p_bar(x ^ 1));
+          else if (more) mbar_arrive(p_bar(x));
+        }
+        commit(more ? s_bar(x) : o_bar(x));
+        commit(empty_bar(v_slot));
+        if (more) {
+          commit(empty_bar(slot));
+          next();
+        }
+      }
+    }
+    // slots that only the other tile works on
+    for (int i = 2 * mine; ok && i < 2 * steps; ++i) {
+      ok = wait(full_bar(slot), phase, 62);
+      if (ok && leader) mbar_arrive(empty_bar(slot));
+      next();
+    }
+    if (!ok)
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    __syncwarp();
+  };
 
   if (warp == W_LOAD) {
     // ------------------------------------------------------------------ loads
@@ -248,92 +345,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);   // let copies in flight land before the block retires
     }
     __syncwarp();
-  } else if (warp == W_MMA || warp == W_MMA + 1) {
-    // ------------------------------------------------------------------ MMAs of one tile
-    // The whole warp runs this code with the same values, one lane issues: operands then live in uniform registers.  With a
-    // single lane in the branch each MMA costs a dozen instructions, and the warp shares its scheduler with busy ones.
-    const int x = warp - W_MMA, mine = __shfl_sync(0xffffffffu, n_x[x], 0), other = __shfl_sync(0xffffffffu, n_x[x ^ 1], 0);
-    const int steps = max(mine, other);
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    const bool leader = lane == 0;
-    auto wait = [&](uint32_t bar, uint32_t phase, int site) {
-      const bool ok = __all_sync(0xffffffffu, wait_bar(bar, phase, abort_flag, a.status, site));
-      tc_fence_after_sync();
-      return ok;
-    };
-    auto commit = [&](uint32_t bar) {
-      if (leader) mma_commit(bar);
-    };
-    const uint32_t s_tmem = tm + 128u * x, o_tmem = tm + 256u + uint32_t(D) * x;
-    const uint64_t qd = make_smem_desc_sw128(q_smem + x * Sh::TILE, 16u, 1024u);
-    const uint64_t ring_k = make_smem_desc_sw128(ring, 16u, 1024u);
-    // V [key][element]: element-major operand, 64-element atoms 16 KB apart, 8 keys 1 KB apart
-    const uint64_t ring_v = make_smem_desc_sw128(ring, 16384u, 1024u);
-    auto scores = [&](int slot, int from, int to) {
-      const uint64_t kd = ring_k + uint64_t(slot * (Sh::TILE / 16));
-#pragma unroll
-      for (int s = from; s < to; ++s) {   // 16 elements = 32 bytes; the next 64 elements lie 16 KB further
-        const uint64_t o = uint64_t((s >> 2) * 1024 + (s & 3) * 2);
-        mma_f16_ss(s_tmem, qd + o, kd + o, p.idesc_s, s > 0, leader);
-      }
-    };
-    auto values = [&](int slot, bool first) {
-      const uint64_t vd = ring_v + uint64_t(slot * (Sh::TILE / 16));
-#pragma unroll
-      for (int s = 0; s < 8; ++s)          // 16 keys = 8 columns of P, 2 KB of V
-        mma_f16_ts(o_tmem, s_tmem + 8u * s, vd + uint64_t(s * 128), p.idesc_o, !(first && s == 0), leader);
-    };
-    bool ok = true;
-    int slot = 0;            // of K(j), then of V(j): slots are taken in the order K(0) V(0) K(1) ...
-    uint32_t phase = 0;
-    auto next = [&] {
-      if (++slot == Sh::SLOTS) slot = 0, phase ^= 1u;
-    };
-    if (mine > 0) {
-      ok = wait(q_bar, 0, 63) && wait(full_bar(0), 0, 62);
-      if (ok) {
-        scores(0, 0, D / 16);
-        commit(s_bar(x));
-        commit(empty_bar(0));
-        if (leader && (x == 0 || other == 0)) mbar_arrive(p_bar(x));   // the first turn
-      }
-      next();
-      for (int j = 0; ok && j < mine; ++j) {
-        const bool more = j + 1 < mine;
-        const int v_slot = slot;
-        ok = wait(full_bar(v_slot), phase, 62);
-        next();
-        if (ok && more) ok = wait(full_bar(slot), phase, 62);
-        // The weights are there and it is this tile's turn: A B A B ...  Were the tiles' MMAs mixed, both would end late and
-        // both softmaxes run while the tensor cores idle.  The ninth arrival at the barrier is the other tile's thread
-        // passing the turn on, or this one where the other tile has no such step.
-        if (ok) ok = wait(p_bar(x), j & 1, 65);
-        if (!ok) break;
-        values(v_slot, j == 0);
-        if (more) scores(slot, 0, TC_EARLY);
-        if (leader) {
-          const int next = x == 0 ? j : j + 1;   // the other tile's step whose turn it is now, if there is one
-          if (next < other) mbar_arrive(p_bar(x ^ 1));
-          else if (more) mbar_arrive(p_bar(x));
-        }
-        if (more) scores(slot, TC_EARLY, D / 16);
-        commit(more ? s_bar(x) : o_bar(x));
-        commit(empty_bar(v_slot));
-        if (more) {
-          commit(empty_bar(slot));
-          next();
-        }
-      }
-    }
-    // slots that only the other tile works on
-    for (int i = 2 * mine; ok && i < 2 * steps; ++i) {
-      ok = wait(full_bar(slot), phase, 62);
-      if (ok && leader) mbar_arrive(empty_bar(slot));
-      next();
-    }
-    if (!ok)
-      for (int i = 0; i < 64; ++i) __nanosleep(1000);
-    __syncwarp();
+  } else if (warp == W_MMA) {
+    mma_role(std::integral_constant<int, 0>());
+  } else if (warp == W_MMA + 1) {
+    mma_role(std::integral_constant<int, 1>());
   } else if (warp == W_EDGE) {
     // ------------------------------------------------------------------ V at the edge
     for (int j = edge0; j < n; ++j) {
@@ -371,80 +386,76 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     volatile float* from = half_row + (2 * x + (half ^ 1)) * 128 + row;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
+    const f2 c2 = pack_f2(c, c);
     for (int j = 0; j < n_x[x]; ++j) {
       ok = wait_bar(s_bar(x), j & 1, abort_flag, a.status, 67);
       tc_fence_after_sync();
-      uint32_t s[64];
-      tmem_ld_32x32(s_tmem + 64u * half, *reinterpret_cast<uint32_t(*)[32]>(s));
-      tmem_ld_32x32(s_tmem + 64u * half + 32u, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
-      tmem_ld_wait();
       const int see = lim - 128 * j - 64 * half;
       const bool masked = __any_sync(0xffffffffu, see < 64);
-      if (masked) {
+      // Weights relative to the maximum so far, and this tile's maximum beside them: the maximum nearly always stays, so the
+      // exponentials need not wait for it.  Where it moves (the first tile always), once more with the new one; S is still
+      // there, P is not stored before the row's two threads agree.
+      for (int attempt = 0;; ++attempt) {
+        const float off = m == -INFINITY ? 0.0f : m;
+        const f2 off2 = pack_f2(-off, -off);
+        float t[2] = {-INFINITY, -INFINITY};
+        f2 sum[2] = {0, 0};
+        uint32_t s[2][16], w[32];   // 16 scores at a time, the next 16 on their way: room for exponentials in flight
+        tmem_ld_32x16(s_tmem + 64u * half, s[0]);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) s[i] = i < see ? s[i] : 0xff800000u;
-      }
-      float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < 64; i += 2) t[(i >> 1) & 3] = max3(t[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-      float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-      *to = top;
-      // the other half's maximum; behind this point both halves have read S, so P may overwrite it
-      ok = all_of(1 + x, 256, ok);
-      if (!ok) break;
-      top = fmaxf(top, *from) * c;
-      if (j == 0) {
-        m = top;
-      } else if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-        const float mn = fmaxf(m, top), alpha = m == mn ? 1.0f : ex2(m - mn);
-        l *= alpha;
-        m = mn;
-#pragma unroll
-        for (int h = 0; h < D / 32; ++h) {   // this half's elements, 16 at a time
-          uint32_t o[16];
-          tmem_ld_32x16(o_tmem + 16u * h, o);
+        for (int h = 0; h < 4; ++h) {
+          uint32_t(&v)[16] = s[h & 1];
           tmem_ld_wait();
+          if (h < 3) tmem_ld_32x16(s_tmem + 64u * half + 16u * (h + 1), s[(h + 1) & 1]);
+          if (masked) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st_32x16(o_tmem + 16u * h, o);
-        }
-      }
-      const float off = m == -INFINITY ? 0.0f : m;
-      const f2 c2 = pack_f2(c, c), off2 = pack_f2(-off, -off);
-      f2 sum[2] = {0, 0};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[16];
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int at = 32 * h + 2 * i;
-            const float y0 = fmaf(__uint_as_float(s[at]), c, -off), y1 = fmaf(__uint_as_float(s[at + 1]), c, -off);
-            const f2 e = pack_f2(at < see ? ex2(y0) : 0.0f, at + 1 < see ? ex2(y1) : 0.0f);
-            sum[i & 1] = add_f2(sum[i & 1], e);
-            w[i] = pack2<BF16>(lo_f2(e), hi_f2(e));
+            for (int i = 0; i < 16; ++i) v[i] = 16 * h + i < see ? v[i] : 0xff800000u;
           }
-        } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const f2 y = fma_f2(pack_f2(__uint_as_float(s[32 * h + 2 * i]), __uint_as_float(s[32 * h + 2 * i + 1])), c2, off2);
+          for (int i = 0; i < 8; ++i) {
+            t[i & 1] = max3(t[i & 1], __uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+            const f2 y = fma_f2(pack_f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, off2);
             const f2 e = pack_f2(ex2(lo_f2(y)), ex2(hi_f2(y)));
             sum[i & 1] = add_f2(sum[i & 1], e);
-            w[i] = pack2<BF16>(lo_f2(e), hi_f2(e));
+            w[8 * h + i] = pack2<BF16>(lo_f2(e), hi_f2(e));
           }
         }
-        tmem_st_32x16(s_tmem + 32u * half + 16u * h, w);
+        float top = fmaxf(t[0], t[1]);
+        if (attempt == 0) *to = top;
+        ok = all_of(1 + 4 * x + (warp & 3), 64, ok);   // behind this point both halves have read S
+        if (!ok) break;
+        if (attempt == 0) top = fmaxf(top, *from) * c;
+        if (attempt == 0 && __any_sync(0xffffffffu, top > m + 8.0f)) {
+          const float mn = fmaxf(m, top), alpha = m == mn ? 1.0f : ex2(m - mn);
+          l *= alpha;
+          m = mn;
+          if (j > 0) {
+#pragma unroll
+            for (int h = 0; h < D / 32; ++h) {   // this half's elements, 16 at a time
+              uint32_t o[16];
+              tmem_ld_32x16(o_tmem + 16u * h, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x16(o_tmem + 16u * h, o);
+            }
+          }
+          continue;
+        }
+        tmem_st_32x32(s_tmem + 32u * half, w);
+        sum[0] = add_f2(sum[0], sum[1]);
+        l += lo_f2(sum[0]) + hi_f2(sum[0]);
+        break;
       }
+      if (!ok) break;
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_bar(x));
-      sum[0] = add_f2(sum[0], sum[1]);
-      l += lo_f2(sum[0]) + hi_f2(sum[0]);
     }
     if (ok && n_x[x] > 0) ok = wait_bar(o_bar(x), 0, abort_flag, a.status, 68);
     *to = l;
-    ok = all_of(1 + x, 256, ok);
+    ok = all_of(1 + 4 * x + (warp & 3), 64, ok);
     if (ok) {
       tc_fence_after_sync();
       l += *from;
