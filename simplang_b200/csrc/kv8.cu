@@ -18,7 +18,7 @@ struct Kv8View {
   float* vs;
   const int32_t* table;
   int64_t table_stride;
-  int n_blocks, bt, G, D, pitch;
+  int n_blocks, bt, G, D, pitch, shift;   // bt = 1 << shift
 };
 
 // ------------------------------------------------------------------------------------------------ write
@@ -34,16 +34,48 @@ __device__ __forceinline__ float kv8_magnitude(float x) {
 // x / s to the nearest integer, halves to even, exactly: the product with 1 / s is within one of it, and the remainder
 // x - n s has no rounding error (n <= 127, |x - n s| < 2 s: a multiple of the smaller ulp that fits 24 bits), so it
 // tells which side of a half x lies on.  A plain division would round quotients next to a half onto it.
-__device__ __forceinline__ int kv8_quantise(float x, float s, float inv) {
+// This is the general form; kv8_round4 takes the values that lie clear of halves, which are nearly all.
+__device__ __forceinline__ uint32_t kv8_quantise(float x, float s, float inv) {
   if (s == 0.0f || x != x) return 0;
-  if (fabsf(x) > FLT_MAX) return x > 0.0f ? 127 : -127;
+  if (fabsf(x) > FLT_MAX) return x > 0.0f ? 127u : uint32_t(-127) & 0xffu;
   float n = rintf(x * inv);
   const float r2 = 2.0f * fmaf(-n, s, x);
   if (r2 > s) n += 1.0f;
   else if (r2 < -s) n -= 1.0f;
   else if (fabsf(r2) == s && (int(n) & 1)) n += r2 > 0.0f ? 1.0f : -1.0f;
-  return int(fminf(fmaxf(n, -127.0f), 127.0f));
+  return uint32_t(int(fminf(fmaxf(n, -127.0f), 127.0f))) & 0xffu;
 }
+// (out of line: it is rare, and what a block of few tokens waits for is its instructions)
+__device__ __noinline__ uint32_t kv8_round4_general(float x0, float x1, float x2, float x3, float s, float inv) {
+  return kv8_quantise(x0, s, inv) | kv8_quantise(x1, s, inv) << 8 | kv8_quantise(x2, s, inv) << 16 | kv8_quantise(x3, s, inv) << 24;
+}
+// Four values as four bytes.  Adding 1.5 * 2^23 rounds x / s to an integer that is then the sum's low byte; twice the exact
+// remainder is below `sure` (s, or anything where s is a power of two: the product with 1 / s is then exact and rounded to
+// even) where that integer is the nearest.  Above s it is off by one.  Quotients within rounding of a half are common
+// (half of the largest value is 63.5), exact halves are not but for powers of two, whose blocks are full of them.
+// `odd`: something in the block is not finite, or the step is 0.
+__device__ __forceinline__ uint32_t kv8_round4(const float (&x)[4], float s, float inv, float sure, bool odd) {
+  uint32_t b[4];
+  float r2[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = fmaf(x[i], inv, 12582912.0f), r = fmaf(12582912.0f - t, s, x[i]);
+    r2[i] = r + r;
+    b[i] = __float_as_uint(t);
+  }
+  const float far = fmaxf(fmaxf(fabsf(r2[0]), fabsf(r2[1])), fmaxf(fabsf(r2[2]), fabsf(r2[3])));
+  if (odd || !(far < sure)) {
+    bool half = odd;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      half = half || fabsf(r2[i]) == s;
+      b[i] += uint32_t(r2[i] > s) - uint32_t(r2[i] < -s);
+    }
+    if (half) return kv8_round4_general(x[0], x[1], x[2], x[3], s, inv);
+  }
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ float kv8_sure(float s) { return __float_as_uint(s) & 0x007fffffu ? s : INFINITY; }
 // A held integer to a larger step: q * old is exact in 64 bits, and a quotient that is not a half differs from it by far
 // more than 64-bit rounding.
 __device__ __forceinline__ int kv8_requantise(int q, double old, double now) {
@@ -66,12 +98,12 @@ __device__ __forceinline__ bool kv8_span(const Kv8View& c, int64_t unit, const i
       report_status(status, STATUS_BAD_RANGE, s);
       return 0;
     }
-    return int((st + n - 1) / c.bt - st / c.bt) + 1;
+    return int(((st + n - 1) >> c.shift) - (st >> c.shift)) + 1;
   };
   int place;
   if (!find_unit(unit, n_seqs, count, sp.seq, place)) return false;
   const int q0 = __ldg(off + sp.seq), n = __ldg(off + sp.seq + 1) - q0, st = __ldg(starts + sp.seq);
-  const int64_t bi = st / c.bt + place, p0 = bi * c.bt;
+  const int64_t bi = (st >> c.shift) + place, p0 = bi << c.shift;
   sp.a = int(max(int64_t(st) - p0, int64_t(0)));
   sp.b = int(min(int64_t(st) + n - p0, int64_t(c.bt)));
   sp.row0 = int(q0 + (p0 + sp.a - st));
@@ -83,77 +115,209 @@ __device__ __forceinline__ bool kv8_span(const Kv8View& c, int64_t unit, const i
   return true;
 }
 
-constexpr int KV8_THREADS = 128;
-// One block of 128 threads per (sequence, cache block, head).
-template <typename T>
-__global__ void __launch_bounds__(KV8_THREADS) kv8_append_kernel(Kv8View c, const T* __restrict__ k, const T* __restrict__ v,
-                                                                 int64_t row_stride, const int32_t* __restrict__ off,
-                                                                 const int32_t* __restrict__ starts, int n_seqs, int64_t total,
-                                                                 int* status) {
-  __shared__ float red[33];
+// A thread owns a patch of 16 tokens x 4 elements of K and the same of V: K leaves as words (a warp writes whole rows), V
+// as 16-byte columns.  A block of threads per (sequence, cache block, head): bt / 16 x pitch / 4 patches.  Rows are read
+// twice, for the maximum and for the values; the second time they come from L1.  (Keeping both patches in registers
+// between the passes was tried: 254 registers, and code so long that fetching it took most of the time; 8192 rows of 8
+// heads x 128 took 90 us, one token for each of 48 sequences 39.)
+// VEC: four elements lie together at a multiple of their size (head_dim a multiple of 4, aligned pointers and stride).
+// Four elements as they are stored: what the maximum is taken of, two 16-bit ones at a time.
+template <typename T> struct Kv8Raw;
+template <> struct Kv8Raw<float> {
+  uint32_t w[4];
+  __device__ __forceinline__ void top(uint32_t& t) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t = max(t, w[i] & 0x7fffffffu);
+  }
+  static __device__ __forceinline__ float magnitude(uint32_t t) { return __uint_as_float(t); }   // may be infinity or NaN
+};
+template <typename T> struct Kv8Raw {
+  uint32_t w[2];
+  __device__ __forceinline__ void top(uint32_t& t) const {
+    asm("max.u16x2 %0, %0, %1;" : "+r"(t) : "r"(w[0] & 0x7fff7fffu));
+    asm("max.u16x2 %0, %0, %1;" : "+r"(t) : "r"(w[1] & 0x7fff7fffu));
+  }
+  static __device__ __forceinline__ float magnitude(uint32_t t) {
+    const uint16_t m = uint16_t(max(t & 0xffffu, t >> 16));
+    return to_f32(reinterpret_cast<const T&>(m));
+  }
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ Kv8Raw<T> kv8_raw4(const T* row, int d, int D) {
+  Kv8Raw<T> r;
+  if (VEC) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(r.w) = *reinterpret_cast<const uint4*>(row + d);
+    else *reinterpret_cast<uint2*>(r.w) = *reinterpret_cast<const uint2*>(row + d);
+  } else {
+    T* e = reinterpret_cast<T*>(r.w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = d + i < D ? row[d + i] : from_f32<T>(0.0f);
+  }
+  return r;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void kv8_load4(const T* row, int d, int D, float (&x)[4]) {
+  const Kv8Raw<T> r = kv8_raw4<T, VEC>(row, d, D);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = to_f32(reinterpret_cast<const T*>(r.w)[i]);
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void kv8_store4(T* row, int d, int D, const float (&x)[4]) {
+  if (VEC) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(row + d) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+      uint2 w;
+      T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(x[i]);
+      *reinterpret_cast<uint2*>(row + d) = w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < D) row[d + i] = from_f32<T>(x[i]);
+  }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) kv8_append_kernel(Kv8View c, const T* __restrict__ k, const T* __restrict__ v,
+                                                         int64_t row_stride, const int32_t* __restrict__ off,
+                                                         const int32_t* __restrict__ starts, int n_seqs, int64_t total, int* status) {
+  __shared__ float tops[2][8];
   Kv8Span sp;
   if (!kv8_span(c, blockIdx.x, off, starts, n_seqs, total, status, sp)) return;
-  const int h = blockIdx.y, n_new = sp.b - sp.a;
-  const T* kr = k + int64_t(sp.row0) * row_stride + int64_t(h) * c.D;
-  const T* vr = v + int64_t(sp.row0) * row_stride + int64_t(h) * c.D;
+  const int h = blockIdx.y, quads = c.pitch >> 2, g = threadIdx.x / quads, d = 4 * (threadIdx.x % quads);
+  const int t0 = 16 * g, lo = max(sp.a - t0, 0), hi = g < (c.bt >> 4) ? min(sp.b - t0, 16) : 0;   // new tokens of the patch: [lo, hi)
+  const int64_t at = (int64_t(sp.row0) + t0 - sp.a) * row_stride + int64_t(h) * c.D;
+  const bool some = d < c.D;   // pad elements are written as zeros
+  const T *kr = k + at, *vr = v + at;
   const int64_t sc = int64_t(sp.block) * c.G + h;
-  float topk = 0.0f, topv = 0.0f;
-  for (int i = threadIdx.x; i < n_new * c.D; i += KV8_THREADS) {
-    const int r = i / c.D, d = i - r * c.D;
-    topk = fmaxf(topk, kv8_magnitude(to_f32(kr[r * row_stride + d])));
-    topv = fmaxf(topv, kv8_magnitude(to_f32(vr[r * row_stride + d])));
-  }
   const float old_k = sp.a ? c.ks[sc] : 0.0f, old_v = sp.a ? c.vs[sc] : 0.0f;
-  topk = block_max(topk, red);
-  topv = block_max(topv, red);
-  const float sk = fmaxf(kv8_step(topk), old_k), sv = fmaxf(kv8_step(topv), old_v);
-  const float ik = sk > 0.0f ? 1.0f / sk : 0.0f, iv = sv > 0.0f ? 1.0f / sv : 0.0f;
-  int8_t* kb = c.k + sc * c.bt * c.pitch;
-  int8_t* vb = c.v + sc * c.bt * c.pitch;
-  if (sp.a && sk != old_k)
-    for (int i = threadIdx.x; i < sp.a * c.pitch; i += KV8_THREADS) kb[i] = int8_t(kv8_requantise(kb[i], old_k, sk));
-  for (int i = threadIdx.x; i < n_new * c.pitch; i += KV8_THREADS) {
-    const int r = i / c.pitch, d = i - r * c.pitch;
-    kb[(sp.a + r) * c.pitch + d] = d < c.D ? int8_t(kv8_quantise(to_f32(kr[r * row_stride + d]), sk, ik)) : int8_t(0);
+  uint32_t tk = 0, tv = 0;
+  if (some) {
+#pragma unroll 4
+    for (int j = lo; j < hi; ++j) {
+      kv8_raw4<T, VEC>(kr + j * row_stride, d, c.D).top(tk);
+      kv8_raw4<T, VEC>(vr + j * row_stride, d, c.D).top(tv);
+    }
   }
-  const bool grew = sp.a && sv != old_v;
-  const int g0 = grew ? 0 : sp.a >> 4, g1 = (sp.b + 15) >> 4;
-  for (int i = threadIdx.x; i < (g1 - g0) * c.pitch; i += KV8_THREADS) {
-    const int g = g0 + i / c.pitch, d = i % c.pitch;
-    int8_t* p = vb + (int64_t(g) * c.pitch + d) * 16;
-    for (int j = 0; j < 16; ++j) {
-      const int t = 16 * g + j;
-      if (t < sp.a) {
-        if (grew) p[j] = int8_t(kv8_requantise(p[j], old_v, sv));
-      } else if (t < sp.b) {
-        p[j] = d < c.D ? int8_t(kv8_quantise(to_f32(vr[(t - sp.a) * row_stride + d]), sv, iv)) : int8_t(0);
+  float topk = Kv8Raw<T>::magnitude(tk), topv = Kv8Raw<T>::magnitude(tv);
+  const bool odd = __syncthreads_or(!(topk <= FLT_MAX) || !(topv <= FLT_MAX));
+  if (odd) {   // infinities and NaN do not count
+    topk = topv = 0.0f;
+#pragma unroll 1
+    for (int j = lo; some && j < hi; ++j) {
+      float x[4], y[4];
+      kv8_load4<T, VEC>(kr + j * row_stride, d, c.D, x);
+      kv8_load4<T, VEC>(vr + j * row_stride, d, c.D, y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        topk = fmaxf(topk, kv8_magnitude(x[i]));
+        topv = fmaxf(topv, kv8_magnitude(y[i]));
       }
     }
   }
-  if (threadIdx.x == 0) {
+  topk = warp_max(topk);
+  topv = warp_max(topv);
+  if ((threadIdx.x & 31) == 0) {
+    tops[0][threadIdx.x >> 5] = topk;
+    tops[1][threadIdx.x >> 5] = topv;
+  }
+  __syncthreads();
+  for (int i = 0; i < int(blockDim.x >> 5); ++i) {
+    topk = fmaxf(topk, tops[0][i]);
+    topv = fmaxf(topv, tops[1][i]);
+  }
+  const float sk = fmaxf(kv8_step(topk), old_k), sv = fmaxf(kv8_step(topv), old_v);
+  if (threadIdx.x == 0) {   // every thread has read the old scales: they were loaded before the barrier
     c.ks[sc] = sk;
     c.vs[sc] = sv;
+  }
+  const bool grew_k = sp.a && sk != old_k, grew_v = sp.a && sv != old_v;
+  if (g >= (c.bt >> 4)) return;
+  const float ik = sk > 0.0f ? 1.0f / sk : 0.0f, iv = sv > 0.0f ? 1.0f / sv : 0.0f;
+  const float sure_k = kv8_sure(sk), sure_v = kv8_sure(sv);
+  int8_t* kb = c.k + sc * c.bt * c.pitch + int64_t(t0) * c.pitch + d;
+  int8_t* vb = c.v + sc * c.bt * c.pitch + (int64_t(g) * c.pitch + d) * 16;
+  const int held = min(lo, 16);   // tokens of the patch that the block held before
+  if (grew_k)
+#pragma unroll 1
+    for (int i = 0; i < 4 * held; ++i) kb[(i >> 2) * c.pitch + (i & 3)] = int8_t(kv8_requantise(kb[(i >> 2) * c.pitch + (i & 3)], old_k, sk));
+  if (grew_v)
+#pragma unroll 1
+    for (int i = 0; i < 4 * held; ++i) vb[16 * (i & 3) + (i >> 2)] = int8_t(kv8_requantise(vb[16 * (i & 3) + (i >> 2)], old_v, sv));
+#pragma unroll 4
+  for (int j = lo; j < hi; ++j) {
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (some) kv8_load4<T, VEC>(kr + j * row_stride, d, c.D, x);
+    *reinterpret_cast<uint32_t*>(kb + j * c.pitch) = kv8_round4(x, sk, ik, sure_k, odd || sk == 0.0f);
+  }
+  if (lo == 0 && hi == 16) {
+    uint32_t col[4][4];   // element, four words of four tokens
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      uint32_t r[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (some) kv8_load4<T, VEC>(vr + (4 * w + j) * row_stride, d, c.D, x);
+        r[j] = kv8_round4(x, sv, iv, sure_v, odd || sv == 0.0f);
+      }
+      // rows of four elements to columns of four tokens
+      const uint32_t p0 = __byte_perm(r[0], r[1], 0x5140), p1 = __byte_perm(r[0], r[1], 0x7362);
+      const uint32_t q0 = __byte_perm(r[2], r[3], 0x5140), q1 = __byte_perm(r[2], r[3], 0x7362);
+      col[0][w] = __byte_perm(p0, q0, 0x5410);
+      col[1][w] = __byte_perm(p0, q0, 0x7632);
+      col[2][w] = __byte_perm(p1, q1, 0x5410);
+      col[3][w] = __byte_perm(p1, q1, 0x7632);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(vb)[i] = make_uint4(col[i][0], col[i][1], col[i][2], col[i][3]);
+  } else {   // part of a column: byte by byte, what lies before and behind the new tokens stays
+#pragma unroll 1
+    for (int j = lo; j < hi; ++j) {
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (some) kv8_load4<T, VEC>(vr + j * row_stride, d, c.D, x);
+      const uint32_t r = kv8_round4(x, sv, iv, sure_v, odd || sv == 0.0f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vb[16 * i + j] = int8_t(r >> (8 * i));
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ read
-template <typename T>
-__global__ void __launch_bounds__(KV8_THREADS) kv8_read_kernel(Kv8View c, T* __restrict__ k, T* __restrict__ v, int64_t row_stride,
-                                                               const int32_t* __restrict__ off, const int32_t* __restrict__ starts,
-                                                               int n_seqs, int64_t total, int* status) {
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) kv8_read_kernel(Kv8View c, T* __restrict__ k, T* __restrict__ v, int64_t row_stride,
+                                                       const int32_t* __restrict__ off, const int32_t* __restrict__ starts,
+                                                       int n_seqs, int64_t total, int* status) {
   Kv8Span sp;
   if (!kv8_span(c, blockIdx.x, off, starts, n_seqs, total, status, sp)) return;
-  const int h = blockIdx.y, n = sp.b - sp.a;
+  const int h = blockIdx.y, quads = c.pitch >> 2, g = threadIdx.x / quads, d = 4 * (threadIdx.x % quads);
+  const int t0 = 16 * g, lo = max(sp.a - t0, 0), hi = g < (c.bt >> 4) ? min(sp.b - t0, 16) : 0;
+  if (hi <= lo || d >= c.D) return;
   const int64_t sc = int64_t(sp.block) * c.G + h;
-  const float sk = c.ks[sc], sv = c.vs[sc];
-  const int8_t* kb = c.k + sc * c.bt * c.pitch;
-  const int8_t* vb = c.v + sc * c.bt * c.pitch;
-  T* kr = k + int64_t(sp.row0) * row_stride + int64_t(h) * c.D;
-  T* vr = v + int64_t(sp.row0) * row_stride + int64_t(h) * c.D;
-  for (int i = threadIdx.x; i < n * c.D; i += KV8_THREADS) {
-    const int r = i / c.D, d = i - r * c.D, t = sp.a + r;
-    kr[r * row_stride + d] = from_f32<T>(float(kb[t * c.pitch + d]) * sk);
-    vr[r * row_stride + d] = from_f32<T>(float(vb[(int64_t(t >> 4) * c.pitch + d) * 16 + (t & 15)]) * sv);
+  const float sk = __ldg(c.ks + sc), sv = __ldg(c.vs + sc);
+  const int8_t* kb = c.k + sc * c.bt * c.pitch + int64_t(t0) * c.pitch + d;
+  const uint4* vb = reinterpret_cast<const uint4*>(c.v + sc * c.bt * c.pitch) + int64_t(g) * c.pitch + d;
+  uint32_t kw[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) kw[j] = __ldcs(reinterpret_cast<const uint32_t*>(kb + j * c.pitch));
+  uint4 vw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) vw[i] = __ldcs(vb + i);
+  const int64_t at = (int64_t(sp.row0) + t0 - sp.a) * row_stride + int64_t(h) * c.D;
+  auto byte_of = [](uint32_t w, int i) { return float(int8_t(uint8_t(w >> (8 * i)))); };
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    if (j < lo || j >= hi) continue;
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = byte_of(kw[j], i) * sk;
+    kv8_store4<T, VEC>(k + at + j * row_stride, d, c.D, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = byte_of((&vw[i].x)[j >> 2], j & 3) * sv;
+    kv8_store4<T, VEC>(v + at + j * row_stride, d, c.D, x);
   }
 }
 
@@ -298,12 +462,11 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
 
   const int c0 = chunk * a.chunk, c1 = min(len, c0 + a.chunk);
   const int32_t* table = a.c.table + s * c.table_stride;
-  const int bt_shift = 31 - __clz(c.bt);
   const int64_t head_bytes = int64_t(c.bt) * P;
   // block of the 16 tokens from `tok` on; tokens behind the sequence use the block of the tile's first token
   auto entry = [&](int tile, int half) {
     const int tok = tile + 16 * half;
-    return __ldg(table + ((tok < len ? tok : tile) >> bt_shift));
+    return __ldg(table + ((tok < len ? tok : tile) >> c.shift));
   };
   for (int tile = c0 + 32 * warp; tile < c1; tile += 32 * AK_WARPS) {
     int be = entry(tile, g >> 2), bv = entry(tile, t >> 1);
@@ -518,7 +681,7 @@ static int kv8_check(const char* who, const simp_kv8_cache* c, const int32_t* ta
   SIMP_REQUIRE(aligned_to(c->k, 16) && aligned_to(c->v, 16), SIMP_ERR_ARG, "%s: the cache's k and v must be 16-byte aligned", who);
   SIMP_REQUIRE(table_stride >= 1 && table_stride <= INT_MAX / c->block_tokens, SIMP_ERR_SHAPE, "%s: table_stride %lld", who, (long long)table_stride);
   v = Kv8View{c->k, c->v, c->k_scales, c->v_scales, table, table_stride, int(c->n_blocks), int(c->block_tokens), int(c->n_kv_heads),
-              int(c->head_dim), int((c->head_dim + 31) / 32 * 32)};
+              int(c->head_dim), int((c->head_dim + 31) / 32 * 32), 31 - __builtin_clz(unsigned(c->block_tokens))};
   return SIMP_OK;
 }
 
@@ -541,12 +704,18 @@ static int kv8_rows(const char* who, bool write, const simp_kv8_cache* cache, co
   // a sequence of n rows touches at most (n - 1) / bt + 2 blocks, and never more than n
   const dim3 grid(unsigned(std::min<int64_t>(total, total / c.bt + 2 * n_seqs)), unsigned(c.G));
   int* status = ctx().dev_status;
+  const unsigned threads = unsigned((c.bt / 16 * (c.pitch / 4) + 31) / 32 * 32);
+  const size_t four = 4 * dtype_size(dtype);
+  const bool vec = c.D % 4 == 0 && kv_stride % 4 == 0 && aligned_to(k, four) && aligned_to(v, four);
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    if (write)
-      kv8_append_kernel<T><<<grid, KV8_THREADS, 0, st>>>(c, static_cast<const T*>(k), static_cast<const T*>(v), kv_stride, off, starts, int(n_seqs), total, status);
-    else
-      kv8_read_kernel<T><<<grid, KV8_THREADS, 0, st>>>(c, static_cast<T*>(k), static_cast<T*>(v), kv_stride, off, starts, int(n_seqs), total, status);
+    if (write) {
+      auto kern = vec ? kv8_append_kernel<T, true> : kv8_append_kernel<T, false>;
+      kern<<<grid, threads, 0, st>>>(c, static_cast<const T*>(k), static_cast<const T*>(v), kv_stride, off, starts, int(n_seqs), total, status);
+    } else {
+      auto kern = vec ? kv8_read_kernel<T, true> : kv8_read_kernel<T, false>;
+      kern<<<grid, threads, 0, st>>>(c, static_cast<T*>(k), static_cast<T*>(v), kv_stride, off, starts, int(n_seqs), total, status);
+    }
   };
   if (dtype == SIMP_DTYPE_F32) go(float());
   else if (dtype == SIMP_DTYPE_F16) go(__half());

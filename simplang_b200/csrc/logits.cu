@@ -26,7 +26,8 @@ struct LogitsArgs {
 
 constexpr int LG_THREADS = 256;
 
-// Larger floats have larger keys, equal ones the larger key at the lower index.  Never 0.
+// Larger floats have larger keys, equal ones the larger key at the lower index.  Never 0, and only asked for values above
+// -infinity.
 __device__ __forceinline__ unsigned long long logit_key(float v, int i) {
   uint32_t b = __float_as_uint(v == 0.0f ? 0.0f : v);   // -0 and 0 are equal
   b = b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -37,19 +38,19 @@ __device__ __forceinline__ unsigned long long logit_key(float v, int i) {
 template <typename T, int U>
 __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) {
   constexpr int VEC = 16 / sizeof(T), SEG = LG_THREADS * U * VEC;
-  extern __shared__ int lg_smem[];
+  extern __shared__ __align__(16) int lg_smem[];
   __shared__ unsigned long long wbest[LG_THREADS / 32];
   const int row = blockIdx.y;
   const T* in = static_cast<const T*>(a.in) + row * a.stride;
   T* out = static_cast<T*>(a.out) + row * a.stride;
   // segments start on 16-byte boundaries of the input: token `base` may lie before the row, by less than a vector
   const int mis = int((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
-  const int64_t base = int64_t(blockIdx.x) * SEG - mis;
+  const int base = int(blockIdx.x) * SEG - mis;
   const bool st16 = (reinterpret_cast<uintptr_t>(out + base) & 15) == 0;
   T x[U][VEC];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t v0 = base + int64_t(u * LG_THREADS + threadIdx.x) * VEC;
+    const int v0 = base + (u * LG_THREADS + threadIdx.x) * VEC;
     if (v0 >= 0 && v0 + VEC <= a.vocab) {
       *reinterpret_cast<uint4*>(x[u]) = *reinterpret_cast<const uint4*>(in + v0);
     } else {
@@ -62,20 +63,21 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
   int* bias = lg_smem + (a.r.tokens ? SEG : 0);
   if (a.r.tokens || a.r.bias_tokens) {
     if (a.r.tokens)
-      for (int i = threadIdx.x; i < SEG; i += LG_THREADS) count[i] = 0;
+      for (int i = 4 * threadIdx.x; i < SEG; i += 4 * LG_THREADS) *reinterpret_cast<int4*>(count + i) = make_int4(0, 0, 0, 0);
     if (a.r.bias_tokens)
-      for (int i = threadIdx.x; i < SEG; i += LG_THREADS) bias[i] = -1;
+      for (int i = 4 * threadIdx.x; i < SEG; i += 4 * LG_THREADS) *reinterpret_cast<int4*>(bias + i) = make_int4(-1, -1, -1, -1);
     __syncthreads();
     int b, e;
+    const int first = max(base, 0), last = min(base + SEG, a.vocab);
     if (a.r.tokens && seq_range(a.r.token_offsets, row, a.r.n_tokens, a.status, b, e))
-      for (int i = b + threadIdx.x; i < e; i += LG_THREADS) {
+      for (int i = b + int(threadIdx.x); i < e; i += LG_THREADS) {
         const int id = __ldg(a.r.tokens + i);
-        if (id >= 0 && id < a.vocab && id - base >= 0 && id - base < SEG) atomicAdd(count + (id - base), 1);
+        if (id >= first && id < last) atomicAdd(count + (id - base), 1);
       }
     if (a.r.bias_tokens && seq_range(a.r.bias_offsets, row, a.r.n_bias, a.status, b, e))
       for (int i = b + threadIdx.x; i < e; i += LG_THREADS) {
         const int id = __ldg(a.r.bias_tokens + i);
-        if (id >= 0 && id < a.vocab && id - base >= 0 && id - base < SEG) atomicMax(bias + (id - base), i);   // the last entry wins
+        if (id >= first && id < last) atomicMax(bias + (id - base), i);   // the last entry wins
       }
     __syncthreads();
   }
@@ -83,37 +85,58 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
   const float freq = a.r.frequency ? __ldg(a.r.frequency + row) : 0.0f;
   const float pres = a.r.presence ? __ldg(a.r.presence + row) : 0.0f;
   const uint32_t* mask = a.r.allowed ? a.r.allowed + row * a.r.allowed_stride : nullptr;
-  unsigned long long top = 0;
+  float top_v = -INFINITY;   // a thread's tokens ascend, so the first of equals stays
+  int top_i = -1;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int l0 = (u * LG_THREADS + threadIdx.x) * VEC;
-    const int64_t v0 = base + l0;
+    const int l0 = (u * LG_THREADS + threadIdx.x) * VEC, v0 = base + l0;
+    float f[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = to_f32(x[u][j]);
+    if (a.r.tokens) {
+      int n[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4) *reinterpret_cast<int4*>(n + j) = *reinterpret_cast<const int4*>(count + l0 + j);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (n[j] > 0) {   // separate roundings, so that the result does not hang on a contraction
+          f[j] = f[j] > 0.0f ? __fdiv_rn(f[j], rep) : __fmul_rn(f[j], rep);
+          f[j] = __fsub_rn(f[j], __fadd_rn(__fmul_rn(freq, float(n[j])), pres));
+        }
+    }
+    if (a.r.bias_tokens) {
+      int e[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4) *reinterpret_cast<int4*>(e + j) = *reinterpret_cast<const int4*>(bias + l0 + j);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (e[j] >= 0) f[j] = __fadd_rn(f[j], __ldg(a.r.bias_values + e[j]));
+    }
+    const bool whole = v0 >= 0 && v0 + VEC <= a.vocab;
+    if (mask) {
+      // a vector's bits lie in one word or two: 64 bits from the word of its first token on
+      const int w0 = max(v0, 0) >> 5, w1 = min(w0 + 1, (a.vocab - 1) >> 5);
+      if (v0 < a.vocab) {
+        const uint32_t lo = __ldg(mask + w0), hi = __ldg(mask + w1);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const int at = v0 + j - 32 * w0;   // negative before the row: that token is not written
+          const uint32_t bit = at < 32 ? lo >> (at & 31) : hi >> (at & 31);
+          if (!(bit & 1u)) f[j] = -INFINITY;
+        }
+      }
+    }
     T y[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const int64_t v = v0 + j;
-      if (v < 0 || v >= a.vocab) continue;
-      float f = to_f32(x[u][j]);
-      if (a.r.tokens) {
-        const int n = count[l0 + j];
-        if (n > 0) {   // separate roundings, so that the result does not hang on a contraction
-          f = f > 0.0f ? __fdiv_rn(f, rep) : __fmul_rn(f, rep);
-          f = __fsub_rn(f, __fadd_rn(__fmul_rn(freq, float(n)), pres));
-        }
-      }
-      if (a.r.bias_tokens) {
-        const int e = bias[l0 + j];
-        if (e >= 0) f = __fadd_rn(f, __ldg(a.r.bias_values + e));
-      }
-      if (mask && !((__ldg(mask + (v >> 5)) >> (v & 31)) & 1u)) f = -INFINITY;
-      y[j] = from_f32<T>(f);
+      y[j] = from_f32<T>(f[j]);
       const float w = to_f32(y[j]);
-      if (a.best && w == w) {
-        const unsigned long long k = logit_key(w, int(v));
-        top = k > top ? k : top;
+      if (w > top_v && (whole || (v0 + j >= 0 && v0 + j < a.vocab))) {
+        top_v = w;
+        top_i = v0 + j;
       }
     }
-    if (st16 && v0 >= 0 && v0 + VEC <= a.vocab) {
+    if (st16 && whole) {
       *reinterpret_cast<uint4*>(out + v0) = *reinterpret_cast<const uint4*>(y);
     } else {
 #pragma unroll
@@ -122,6 +145,7 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
     }
   }
   if (!a.best) return;
+  unsigned long long top = top_i >= 0 ? logit_key(top_v, top_i) : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const unsigned long long k = __shfl_xor_sync(0xffffffffu, top, o);
@@ -139,8 +163,7 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
     top = atomicExch(a.key + row, 0ull);
     a.arrived[row] = 0;
   }
-  constexpr uint32_t lowest = 0x007fffffu;   // the key of -infinity
-  a.best[row] = uint32_t(top >> 32) > lowest ? int(0xffffffffu - uint32_t(top)) : -1;
+  a.best[row] = top ? int(0xffffffffu - uint32_t(top)) : -1;
 }
 
 template <typename T>
