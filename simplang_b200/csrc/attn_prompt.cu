@@ -232,8 +232,11 @@ SIMP_API int simp_gpu_attn_prompt(const void* q_dev, const void* k_dev, const vo
   a.D = int(head_dim);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = ctx().dev_status;
-  if (attn_prompt_tc_takes(a, dtype)) return attn_prompt_tc(a, dtype);
-  if (dtype == SIMP_DTYPE_F32) return ap_dispatch<float>(a);
+  if (dtype == SIMP_DTYPE_F32) {
+    if (int rc = attn_prompt_f32_tc(a); rc <= 0) return rc;
+    return ap_dispatch<float>(a);
+  }
+  if (int rc = attn_prompt_tc(a, dtype); rc <= 0) return rc;
   if (dtype == SIMP_DTYPE_F16) return ap_dispatch<__half>(a);
   return ap_dispatch<__nv_bfloat16>(a);
 }

@@ -17,7 +17,10 @@ struct AttnPromptArgs {
   int* status;
 };
 
-bool attn_prompt_tc_takes(const AttnPromptArgs& a, int dtype);
-int attn_prompt_tc(const AttnPromptArgs& a, int dtype);
+// Tensor-core forms; 1: the call is not for them (nothing was launched).
+int attn_prompt_tc(const AttnPromptArgs& a, int dtype);    // 16-bit types
+int attn_prompt_f32_tc(const AttnPromptArgs& a);           // f32
+// Rows to padded rows (f32: three bf16 planes), see attn_prompt_tc.cu.
+int attn_pack(bool split, const void* src, void* dst, int64_t rows, int heads, int D, int DP, int64_t stride, uint8_t* odd, int* any);
 
 }  // namespace simp

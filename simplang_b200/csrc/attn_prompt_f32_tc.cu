@@ -1,0 +1,385 @@
+// attn_prompt_f32_tc.cu -- causal attention over packed prompts at f32 accuracy on the tcgen05 tensor cores.
+//
+// q, k and v are split into three bf16 planes each (x = h + m + l, 24 bits), and a product is the six plane products of
+// relative size 2^-16 and above: l.h, h.l, m.m, m.h, h.m, h.h.  The tensor cores add into their f32 accumulators with
+// truncation, so (1) the small products come first and only the last eighth or less of the additions is made at full
+// size, and (2) the output of every tile of 64 keys is a sum of its own, added to f32 registers with rounding: an
+// accumulator kept over a long prompt would drift by 2e-8 per instruction.
+//
+// One block of 12 warps per row tile (128 rows: 128 / rep tokens x the rep heads that share a key/value head):
+//   warp 0      TMA: the planes of Q once, of K and V per tile of 64 keys
+//   warp 1      MMAs: S = Q K^T (128 x 64) as soon as the softmax has read the S before; T = P V into a TMEM tile
+//   warps 4-11  softmax, two threads per row (32 keys each); P in three planes to TMEM; T into registers (D / 2 each)
+// Per tile the tensor cores need 6 x (D / 16 x 48 + 4 x D / 2) cycles (the first is bound by shared memory: 6 KB per 48
+// cycles), for D = 128 3840, the softmax about 2500 beside them.
+//
+// No plane product of an infinity or a NaN is right, and a zero weight does not hide them from an MMA (a tile may hold keys
+// that some rows must not see, or rows of the next sequence).  The splitting pass leaves them out of the planes and marks
+// the row and head; where anything is marked, scores of marked rows are computed again from the f32 tensors, and marked
+// values that a row sees are added to its output at the end.  Whoever does not see them gets the same bits as without.
+#include <algorithm>
+#include <climits>
+
+#include "attn_tc.cuh"
+
+namespace simp {
+
+constexpr int F3_THREADS = 384, F3_KEYS = 64;
+
+template <int D>
+struct F3Shape {
+  static constexpr int QPLANE = 128 * D * 2, KPLANE = F3_KEYS * D * 2;
+  static constexpr int BARS = 9;
+  static constexpr size_t SMEM = 3 * size_t(QPLANE) + 6 * size_t(KPLANE) + BARS * 8 + 16 + 8 * 128;
+  static constexpr uint32_t TMEM = D == 64 ? 256 : 512, P = 64, T = D == 64 ? 160 : 256;   // columns: S at 0, three P planes, T
+};
+static_assert(F3Shape<128>::SMEM <= 232448 && 2 * F3Shape<64>::SMEM <= 228 * 1024 - 2048, "");
+
+struct F3Args {
+  AttnPromptArgs a;
+  int tpt;
+  const int* any;   // set: some element is not finite; then the bytes of its row and head are set:
+  const uint8_t *odd_q, *odd_k, *odd_v;
+};
+
+__device__ __forceinline__ uint32_t tmem_ld_1(uint32_t t) {
+  uint32_t v;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(t) : "memory");
+  return v;
+}
+__device__ __forceinline__ void tmem_st_1(uint32_t t, uint32_t v) { asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(t), "r"(v) : "memory"); }
+
+template <int D>
+__global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
+    attn_prompt_f32_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                              const __grid_constant__ CUtensorMap map_v, const F3Args p) {
+  using Sh = F3Shape<D>;
+  extern __shared__ __align__(1024) uint8_t f3_raw[];
+  const uint32_t base = smem_u32(f3_raw), q_smem = base, k_smem = base + 3 * Sh::QPLANE, v_smem = k_smem + 3 * Sh::KPLANE, bars = v_smem + 3 * Sh::KPLANE;
+  const uint32_t q_bar = bars, k_full = bars + 8, k_empty = bars + 16, v_full = bars + 24, v_empty = bars + 32, s_bar = bars + 40, s_read = bars + 48,
+                 p_bar = bars + 56, t_bar = bars + 64;
+  uint8_t* tail = f3_raw + (bars - base) + Sh::BARS * 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8);
+  float* half_row = reinterpret_cast<float*>(tail + 16);   // [half][row]
+  const AttnPromptArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (base & 1023u) {   // never: the declaration asks for it
+    if (threadIdx.x == 0) report_status(a.status, 1, 70);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(q_bar, 1);
+    mbar_init(k_full, 1);
+    mbar_init(k_empty, 1);
+    mbar_init(v_full, 1);
+    mbar_init(v_empty, 1);
+    mbar_init(s_bar, 1);
+    mbar_init(s_read, 8);
+    mbar_init(p_bar, 8);
+    mbar_init(t_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  // ---- which rows
+  const int g = blockIdx.x % a.G;
+  int seq = 0, place = 0, q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+  auto count = [&](int s) {
+    int b, e;
+    return seq_range(a.q_off, s, a.total_q, a.status, b, e) ? (e - b + p.tpt - 1) / p.tpt : 0;
+  };
+  if (!find_unit(blockIdx.x / a.G, a.n_seqs, count, seq, place)) return;
+  seq_range(a.q_off, seq, a.total_q, a.status, q0, q1);
+  if (!seq_range(a.k_off, seq, a.total_k, a.status, k0, k1)) return;
+  const int nq = q1 - q0, nk = k1 - k0;
+  const int r0 = ((nq + p.tpt - 1) / p.tpt - 1 - place) * p.tpt;   // the longest rows first
+  const int64_t shift = int64_t(nk) - nq;
+  auto sees = [&](int token) { return int(max(int64_t(0), min(int64_t(nk), token + shift + 1))); };
+  const int n = (sees(min(r0 + p.tpt, nq) - 1) + F3_KEYS - 1) / F3_KEYS;
+
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), Sh::TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ loads
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(q_bar, 3 * (D / 64) * uint32_t(p.tpt * a.rep) * 128u);
+      for (int s = 0; s < 3; ++s)
+        for (int b = 0; b < D / 64; ++b)
+          tma_load_3d(q_smem + s * Sh::QPLANE + b * 16384, &map_q, q_bar, 64 * b, g * a.rep, int(s * a.total_q) + q0 + r0);
+      bool ok = true;
+      auto tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, uint32_t empty, int j) {
+        ok = ok && wait_bar(empty, (j & 1) ^ 1, abort_flag, a.status, 71);
+        if (!ok) return;
+        mbar_arrive_expect_tx(full, 3 * Sh::KPLANE);
+        for (int s = 0; s < 3; ++s)
+          for (int b = 0; b < D / 64; ++b)
+            tma_load_3d(dst + s * Sh::KPLANE + b * 8192, map, full, 64 * b, g, int(s * a.total_k) + k0 + F3_KEYS * j);
+      };
+      for (int j = 0; ok && j < n; ++j) {
+        tile(&map_k, k_smem, k_full, k_empty, j);
+        tile(&map_v, v_smem, v_full, v_empty, j);
+      }
+      if (!ok)
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);   // let copies in flight land before the block retires
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMAs (the whole warp with the same values, one lane issues)
+    constexpr uint32_t idesc_s = idesc_f16(true, F3_KEYS, false), idesc_t = idesc_f16(true, D, true);
+    const bool leader = lane == 0;
+    auto wait = [&](uint32_t bar, uint32_t phase, int site) {
+      const bool ok = __all_sync(0xffffffffu, wait_bar(bar, phase, abort_flag, a.status, site));
+      tc_fence_after_sync();
+      return ok;
+    };
+    // planes of the two operands, small products first
+    constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+    auto scores = [&] {
+      const uint64_t qd = make_smem_desc_sw128(q_smem, 16u, 1024u), kd = make_smem_desc_sw128(k_smem, 16u, 1024u);
+#pragma unroll
+      for (int t = 0; t < 6; ++t)
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+          mma_f16_ss(tmem, qd + uint64_t(PA[t] * (Sh::QPLANE / 16) + (s >> 2) * 1024 + (s & 3) * 2),
+                     kd + uint64_t(PB[t] * (Sh::KPLANE / 16) + (s >> 2) * 512 + (s & 3) * 2), idesc_s, t > 0 || s > 0, leader);
+    };
+    auto values = [&] {
+      const uint64_t vd = make_smem_desc_sw128(v_smem, 8192u, 1024u);   // 64-element atoms 8 KB apart, 8 keys 1 KB apart
+#pragma unroll
+      for (int t = 0; t < 6; ++t)
+#pragma unroll
+        for (int s = 0; s < F3_KEYS / 16; ++s)
+          mma_f16_ts(tmem + Sh::T, tmem + Sh::P + 32u * PA[t] + 8u * s, vd + uint64_t(PB[t] * (Sh::KPLANE / 16) + s * 128), idesc_t, t > 0 || s > 0, leader);
+    };
+    bool ok = true;
+    if (n > 0) {
+      ok = wait(q_bar, 0, 72) && wait(k_full, 0, 73);
+      if (ok) {
+        scores();
+        if (leader) {
+          mma_commit(s_bar);
+          mma_commit(k_empty);
+        }
+      }
+    }
+    for (int j = 0; ok && j < n; ++j) {
+      if (j + 1 < n) {
+        ok = wait(k_full, (j + 1) & 1, 74) && wait(s_read, j & 1, 75);
+        if (!ok) break;
+        scores();
+        if (leader) {
+          mma_commit(s_bar);
+          mma_commit(k_empty);
+        }
+      }
+      ok = wait(v_full, j & 1, 76) && wait(p_bar, j & 1, 77);
+      if (!ok) break;
+      values();
+      if (leader) {
+        mma_commit(t_bar);
+        mma_commit(v_empty);
+      }
+    }
+    if (!ok)
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ softmax and sums
+    const int half = (warp - 4) >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
+    const uint32_t s_tmem = tmem + lanes + 32u * half, t_tmem = tmem + Sh::T + lanes + uint32_t(D / 2) * half;
+    const int token = r0 + row / a.rep, head = g * a.rep + row % a.rep;
+    const bool mine = row < p.tpt * a.rep && token < nq;
+    const int lim = mine ? sees(token) : 0;
+    volatile float* to = half_row + half * 128 + row;
+    volatile float* from = half_row + (half ^ 1) * 128 + row;
+    const bool any = __ldcg(p.any) != 0, odd_row = any && mine && p.odd_q[int64_t(q0 + token) * a.H + head];
+    float m = -INFINITY, l = 0.0f, o[D / 2];
+#pragma unroll
+    for (int i = 0; i < D / 2; ++i) o[i] = 0.0f;
+    auto add_tile = [&](float alpha) {   // the tile's sum to the registers, then both to the new maximum
+#pragma unroll
+      for (int h = 0; h < D / 32; ++h) {
+        uint32_t t[16];
+        tmem_ld_32x16(t_tmem + 16u * h, t);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[16 * h + i] = (o[16 * h + i] + __uint_as_float(t[i])) * alpha;
+      }
+    };
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      ok = wait_bar(s_bar, j & 1, abort_flag, a.status, 78) && ok;
+      tc_fence_after_sync();
+      if (any) {   // rare: scores of rows that are not finite, by the f32 tensors
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+          const int key = F3_KEYS * j + 32 * half + i;
+          uint32_t v = tmem_ld_1(s_tmem + i);
+          tmem_ld_wait();
+          if (key < lim && (odd_row || p.odd_k[int64_t(k0 + key) * a.G + g])) {
+            const float* qr = static_cast<const float*>(a.q) + int64_t(q0 + token) * a.q_stride + int64_t(head) * a.D;
+            const float* kr = static_cast<const float*>(a.k) + int64_t(k0 + key) * a.kv_stride + int64_t(g) * a.D;
+            float d = 0.0f;
+#pragma unroll 1
+            for (int e = 0; e < a.D; ++e) d = fmaf(qr[e], kr[e], d);
+            v = __float_as_uint(d);
+          }
+          __syncwarp();
+          tmem_st_1(s_tmem + i, v);
+        }
+        tmem_st_wait();
+      }
+      uint32_t s[32];
+      tmem_ld_32x32(s_tmem, s);
+      tmem_ld_wait();
+      const int see = lim - F3_KEYS * j - 32 * half;
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float y = i < see ? __uint_as_float(s[i]) * a.scale_log2 : -INFINITY;
+        s[i] = __float_as_uint(y);
+        top = fmaxf(top, y);
+      }
+      *to = top;
+      tc_fence_before_sync();
+      ok = all_of(1 + (warp & 3), 64, ok);
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(s_read);
+      const float mn = fmaxf(m, fmaxf(top, *from)), off = mn == -INFINITY ? 0.0f : mn;
+      const float alpha = ex2(m - off);   // 0 for the first tile
+      m = mn;
+      // The tile before: when it is done, its sum is taken and its P may be overwritten.  With D = 64 two blocks share the
+      // SM and 80 registers hold either the planes or what follows, so this comes first; with D = 128 the exponentials do,
+      // beside the MMAs of the tile before.
+      auto take = [&] {
+        if (j == 0) return;
+        ok = __all_sync(0xffffffffu, wait_bar(t_bar, (j - 1) & 1, abort_flag, a.status, 79)) && ok;
+        tc_fence_after_sync();
+        add_tile(alpha);
+      };
+      float sum = 0.0f;
+      auto planes = [&](int i, uint32_t& w0, uint32_t& w1, uint32_t& w2) {   // two weights: three planes
+        const float e0 = ex2(__uint_as_float(s[2 * i]) - off), e1 = ex2(__uint_as_float(s[2 * i + 1]) - off);
+        sum += e0 + e1;
+        w0 = pack2<true>(e0, e1);
+        const float f0 = e0 - __uint_as_float(w0 << 16), f1 = e1 - __uint_as_float(w0 & 0xffff0000u);
+        w1 = pack2<true>(f0, f1);
+        w2 = pack2<true>(f0 - __uint_as_float(w1 << 16), f1 - __uint_as_float(w1 & 0xffff0000u));
+      };
+      const uint32_t p_tmem = tmem + lanes + Sh::P + 16u * half;
+      if (D == 64) {
+        take();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[3][8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) planes(8 * h + i, w[0][i], w[1][i], w[2][i]);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) tmem_st_32x8(p_tmem + 32u * q + 8u * h, w[q]);
+        }
+      } else {
+        uint32_t w[3][16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) planes(i, w[0][i], w[1][i], w[2][i]);
+        take();
+#pragma unroll
+        for (int q = 0; q < 3; ++q) tmem_st_32x16(p_tmem + 32u * q, w[q]);
+      }
+      l = fmaf(l, alpha, sum);
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_bar);
+    }
+    if (ok && n > 0) {
+      ok = __all_sync(0xffffffffu, wait_bar(t_bar, (n - 1) & 1, abort_flag, a.status, 80));
+      tc_fence_after_sync();
+      add_tile(1.0f);
+    }
+    *to = l;
+    ok = all_of(1 + (warp & 3), 64, ok);
+    if (ok && mine) {
+      l += *from;
+      float* out = static_cast<float*>(a.out) + int64_t(q0 + token) * a.out_stride + int64_t(head) * a.D + (D / 2) * half;
+      const int cols = a.D - (D / 2) * half;
+      if (any)
+#pragma unroll 1
+        for (int key = 0; key < lim; ++key) {
+          if (!p.odd_v[int64_t(k0 + key) * a.G + g]) continue;
+          const float* v = static_cast<const float*>(a.v) + int64_t(k0 + key) * a.kv_stride + int64_t(g) * a.D + (D / 2) * half;
+#pragma unroll
+          for (int i = 0; i < D / 2; ++i)
+            if (i < cols && !(fabsf(v[i]) <= 3.402823466e38f)) o[i] += v[i];
+        }
+      const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll
+      for (int i = 0; i < D / 2; i += 4) {
+        float r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = l == 0.0f ? 0.0f : o[i + e] / l;
+        if (vec && i + 4 <= cols) {
+          *reinterpret_cast<float4*>(out + i) = make_float4(r[0], r[1], r[2], r[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e < cols) out[i + e] = r[e];
+        }
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, Sh::TMEM);
+  }
+}
+
+template <int D>
+static int f3_launch(F3Args p, const uint8_t* q, const uint8_t* k, const uint8_t* v) {
+  const AttnPromptArgs& a = p.a;
+  p.tpt = 128 / a.rep;
+  CUtensorMap mq, mk, mv;
+  if (int rc = attn_tensor_map(&mq, true, q, 3 * a.total_q, a.H, D, int64_t(a.H) * D, a.rep, p.tpt)) return rc;
+  if (int rc = attn_tensor_map(&mk, true, k, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, F3_KEYS)) return rc;
+  if (int rc = attn_tensor_map(&mv, true, v, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, F3_KEYS)) return rc;
+  auto kern = attn_prompt_f32_tc_kernel<D>;
+  SIMP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(F3Shape<D>::SMEM)));
+  const int64_t units = std::min(a.total_q, a.total_q / p.tpt + a.n_seqs) * a.G;
+  SIMP_REQUIRE(units <= INT_MAX, SIMP_ERR_SHAPE, "attn_prompt: too many rows and heads");
+  kern<<<unsigned(units), F3_THREADS, F3Shape<D>::SMEM, ctx().stream>>>(mq, mk, mv, p);
+  SIMP_LAUNCH_CHECK();
+  return SIMP_OK;
+}
+
+// 1: the call stays with the FFMA kernel (nothing was launched).
+int attn_prompt_f32_tc(const AttnPromptArgs& a) {
+  if (a.total_k == 0 || 3 * a.total_q > INT_MAX || 3 * a.total_k > INT_MAX) return 1;
+  const int D = a.D <= 64 ? 64 : 128;
+  const size_t nq = size_t(a.total_q) * a.H, nk = size_t(a.total_k) * a.G, pad = 16;
+  uint8_t* s = static_cast<uint8_t*>(scratch((nq + 2 * nk) * D * 6 + 4 * pad + nq + 2 * nk, SCRATCH_ATTN_PACK));
+  if (!s) return 1;
+  uint8_t *q = s, *k = q + nq * D * 6, *v = k + nk * D * 6, *any = v + nk * D * 6, *oq = any + pad, *ok = oq + nq, *ov = ok + nk;
+  F3Args p{};
+  p.a = a;
+  p.any = reinterpret_cast<const int*>(any);
+  p.odd_q = oq;
+  p.odd_k = ok;
+  p.odd_v = ov;
+  int* flag = reinterpret_cast<int*>(any);
+  SIMP_CUDA(cudaMemsetAsync(flag, 0, 4, ctx().stream));
+  if (int rc = attn_pack(true, a.q, q, a.total_q, a.H, a.D, D, a.q_stride, oq, flag)) return rc;
+  if (int rc = attn_pack(true, a.k, k, a.total_k, a.G, a.D, D, a.kv_stride, ok, flag)) return rc;
+  if (int rc = attn_pack(true, a.v, v, a.total_k, a.G, a.D, D, a.kv_stride, ov, flag)) return rc;
+  return D == 64 ? f3_launch<64>(p, q, k, v) : f3_launch<128>(p, q, k, v);
+}
+
+}  // namespace simp

@@ -20,16 +20,13 @@
 // later tokens of the sequence, and rows of the NEXT sequence (or behind the last) where the sequence ends inside the tile.
 // Warp 18 therefore zeroes, in the edge tiles only, V rows behind the sequence and every element that is not finite; a bit
 // per such key tells the epilogue to add those elements (read again from global memory) to the rows that do see the key.
-#include <cuda.h>
 #include <algorithm>
 #include <climits>
 #include <type_traits>
 
-#include "attn_prompt.cuh"
-#include "sm100_ptx.cuh"
+#include "attn_tc.cuh"
 
 namespace simp {
-using namespace ptx;
 
 constexpr int TC_THREADS = 640;
 constexpr int W_LOAD = 0, W_MMA = 1, W_EDGE = 3;   // W_MMA: tile A, W_MMA + 1: tile B; 4 .. 19: softmax
@@ -49,104 +46,13 @@ static_assert(TcShape<128>::SMEM <= 232448 && TcShape<64>::SMEM <= 232448, "");
 struct TcArgs {
   AttnPromptArgs a;
   int tpt;          // tokens per row tile
-  uint32_t idesc_s, idesc_o;
+  const void* q;    // what the maps read: the caller's tensors, or copies padded to D elements per head
+  const void* k;
+  const void* v;
+  int64_t q_stride, kv_stride;
+  bool whole;       // outputs are written 16 bytes at a time: a.D == D, aligned rows
 };
 
-// (executed by a whole warp with the same operands; the lane with `leader` issues)
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc, bool leader) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc)), "r"(uint32_t(leader))
-      : "memory");
-}
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc, bool leader) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc)), "r"(uint32_t(leader))
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(m),
-               "r"(bar), "r"(x), "r"(y), "r"(z)
-               : "memory");
-}
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t t, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(t)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_32x16(uint32_t t, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-      "r"(r[14]), "r"(r[15]), "r"(t)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_32x32(uint32_t t, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-      "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
-      "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(t)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// Bounded wait whose usual path is one try: mbar_wait's look at the abort flag first costs a shared-memory round trip.
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int site) {
-  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort_flag, status, site);
-}
-// Barrier of n threads that returns whether `ok` holds for all of them: the warps of a tile give up together, so none is
-// left waiting at the next one.
-__device__ __forceinline__ bool all_of(int id, int n, bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbarrier.cta.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"(n), "r"(uint32_t(ok))
-      : "memory");
-  return r != 0;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// two f32 in a register pair: the packed f32x2 instructions do two operations in one issue slot
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 pack_f2(float lo, float hi) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float lo_f2(f2 v) { return __uint_as_float(uint32_t(v)); }
-__device__ __forceinline__ float hi_f2(f2 v) { return __uint_as_float(uint32_t(v >> 32)); }
-__device__ __forceinline__ f2 fma_f2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f2 add_f2(f2 a, f2 b) {
-  f2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t r;
-  if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 // bits of the 16-bit halves of w that are infinity or NaN
 template <bool BF16>
 __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
@@ -251,6 +157,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     auto commit = [&](uint32_t bar) {
       if (leader) mma_commit(bar);
     };
+    constexpr uint32_t idesc_s = idesc_f16(BF16, 128, false), idesc_o = idesc_f16(BF16, D, true);
     constexpr uint32_t s_tmem = 128u * x, o_tmem = 256u + uint32_t(D) * x;
     const uint64_t qd = make_smem_desc_sw128(q_smem + x * Sh::TILE, 16u, 1024u);
     const uint64_t ring_k = make_smem_desc_sw128(ring, 16u, 1024u);
@@ -261,14 +168,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {   // 16 elements = 32 bytes; the next 64 elements lie 16 KB further
         const uint64_t o = uint64_t((s >> 2) * 1024 + (s & 3) * 2);
-        mma_f16_ss(s_tmem, qd + o, kd + o, p.idesc_s, s > 0, leader);
+        mma_f16_ss(s_tmem, qd + o, kd + o, idesc_s, s > 0, leader);
       }
     };
     auto values = [&](int slot, bool first) {
       const uint64_t vd = ring_v + uint64_t(slot * (Sh::TILE / 16));
 #pragma unroll
       for (int s = 0; s < 8; ++s)          // 16 keys = 8 columns of P, 2 KB of V
-        mma_f16_ts(o_tmem, s_tmem + 8u * s, vd + uint64_t(s * 128), p.idesc_o, !(first && s == 0), leader);
+        mma_f16_ts(o_tmem, s_tmem + 8u * s, vd + uint64_t(s * 128), idesc_o, !(first && s == 0), leader);
     };
     bool ok = true;
     int slot = 0;            // of K(j), then of V(j): slots are taken in the order K(0) V(0) K(1) ...
@@ -460,7 +367,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       tc_fence_after_sync();
       l += *from;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t(q0 + token) * a.out_stride + int64_t(head) * D + (D / 2) * half) * 2;
+      uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t(q0 + token) * a.out_stride + int64_t(head) * a.D + (D / 2) * half) * 2;
       uint32_t odd = 0;
       for (int e = 0; e < TC_EDGE * 4; ++e) odd |= odd_keys[e];
 #pragma unroll
@@ -476,10 +383,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           if (odd)   // rare: a key of an edge tile has elements that are not finite
             for (int key = 128 * edge0; key < lim; ++key)
               if ((odd_keys[(key - 128 * edge0) >> 5] >> (key & 31)) & 1u) {
-                const uint16_t* v = static_cast<const uint16_t*>(a.v) + int64_t(k0 + key) * a.kv_stride + int64_t(g) * D + (D / 2) * half + 32 * h;
+                const uint16_t* v = static_cast<const uint16_t*>(a.v) + int64_t(k0 + key) * a.kv_stride + int64_t(g) * a.D + (D / 2) * half + 32 * h;
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                  if (odd_halves<BF16>(v[i]) & 0xffffu) {
+                  if ((D / 2) * half + 32 * h + i < a.D && (odd_halves<BF16>(v[i]) & 0xffffu)) {
                     const float f = BF16 ? __uint_as_float(uint32_t(v[i]) << 16) : __half2float(__ushort_as_half(v[i]));
                     o[i] = __float_as_uint(__uint_as_float(o[i]) + f);
                   }
@@ -491,7 +398,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             w.y = pack2<BF16>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
             w.z = pack2<BF16>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
             w.w = pack2<BF16>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
-            *reinterpret_cast<uint4*>(out + 64 * h + 16 * i) = w;
+            if (p.whole) {
+              *reinterpret_cast<uint4*>(out + 64 * h + 16 * i) = w;
+            } else {
+              const uint16_t* e = reinterpret_cast<const uint16_t*>(&w);
+#pragma unroll
+              for (int t = 0; t < 8; ++t)
+                if ((D / 2) * half + 32 * h + 8 * i + t < a.D) reinterpret_cast<uint16_t*>(out + 64 * h + 16 * i)[t] = e[t];
+            }
           }
         }
         __syncwarp();
@@ -506,8 +420,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   }
 }
 
-// [rows, heads, D] of 16-bit elements, rows a stride apart; boxes of 64 elements x box_heads x box_rows, 128-byte swizzle.
-static int tc_map(CUtensorMap* map, bool bf16, const void* p, int64_t rows, int64_t heads, int D, int64_t stride, int box_heads, int box_rows) {
+int attn_tensor_map(CUtensorMap* map, bool bf16, const void* p, int64_t rows, int64_t heads, int D, int64_t stride, int box_heads, int box_rows) {
   typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static const Encode enc = [] {
@@ -527,18 +440,13 @@ static int tc_map(CUtensorMap* map, bool bf16, const void* p, int64_t rows, int6
 }
 
 template <bool BF16, int D>
-static int tc_launch(const AttnPromptArgs& a) {
-  TcArgs p{};
-  p.a = a;
+static int tc_launch(TcArgs p) {
+  const AttnPromptArgs& a = p.a;
   p.tpt = 128 / a.rep;
-  // f32 accumulator; operand type; B of the second product is element-major
-  const uint32_t type = (1u << 4) | (uint32_t(BF16) << 7) | (uint32_t(BF16) << 10) | (8u << 24);
-  p.idesc_s = type | (uint32_t(128 >> 3) << 17);
-  p.idesc_o = type | (1u << 16) | (uint32_t(D >> 3) << 17);
   CUtensorMap mq, mk, mv;
-  if (int rc = tc_map(&mq, BF16, a.q, a.total_q, a.H, D, a.q_stride, a.rep, p.tpt)) return rc;
-  if (int rc = tc_map(&mk, BF16, a.k, a.total_k, a.G, D, a.kv_stride, 1, 128)) return rc;
-  if (int rc = tc_map(&mv, BF16, a.v, a.total_k, a.G, D, a.kv_stride, 1, 128)) return rc;
+  if (int rc = attn_tensor_map(&mq, BF16, p.q, a.total_q, a.H, D, p.q_stride, a.rep, p.tpt)) return rc;
+  if (int rc = attn_tensor_map(&mk, BF16, p.k, a.total_k, a.G, D, p.kv_stride, 1, 128)) return rc;
+  if (int rc = attn_tensor_map(&mv, BF16, p.v, a.total_k, a.G, D, p.kv_stride, 1, 128)) return rc;
   auto kern = attn_prompt_tc_kernel<BF16, D>;
   SIMP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(TcShape<D>::SMEM)));
   const int64_t units = std::min(a.total_q, a.total_q / (2 * p.tpt) + a.n_seqs) * a.G;
@@ -548,15 +456,92 @@ static int tc_launch(const AttnPromptArgs& a) {
   return SIMP_OK;
 }
 
-// Whether the tensor-core kernel can take the call: head size, a positive scale (the maximum of the scores is then the
-// maximum of the scaled ones), and rows that TMA can address.
-bool attn_prompt_tc_takes(const AttnPromptArgs& a, int dtype) {
-  return dtype != SIMP_DTYPE_F32 && (a.D == 64 || a.D == 128) && a.scale_log2 > 0.0f && a.scale_log2 <= 3.0e38f && a.total_k > 0 && aligned_to(a.q, 16) &&
-         aligned_to(a.k, 16) && aligned_to(a.v, 16) && aligned_to(a.out, 16) && a.q_stride % 8 == 0 && a.kv_stride % 8 == 0 && a.out_stride % 8 == 0;
+// Rows to rows of heads padded to DP elements.  16-bit types are copied; f32 is split into three bf16 planes h + m + l (8 bits
+// of mantissa each: exact, but for what lies below 2^-133), one behind the other.  Elements that are not finite have no
+// place there: they are zeros in the planes, the byte of their row and head in `odd` is set, and *any.  A thread writes
+// eight elements, the DP / 8 threads of a head are neighbours in a warp.
+template <bool SPLIT>
+__global__ void __launch_bounds__(256) attn_pack_kernel(const void* __restrict__ src, uint16_t* __restrict__ dst, int64_t rows, int heads, int D,
+                                                        int DP, int64_t stride, uint8_t* __restrict__ odd, int* any) {
+  const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;   // eighth of a padded row
+  const int eighths = DP / 8, per = heads * eighths;
+  const int64_t row = i / per;
+  const bool in = row < rows;
+  const int at = int(i - row * per), head = at / eighths, d0 = 8 * (at % eighths);
+  const int64_t from = row * stride + int64_t(head) * D + d0;
+  const int n = in ? min(8, D - d0) : 0;
+  uint4 out[3];
+  uint16_t* h = reinterpret_cast<uint16_t*>(out);
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (SPLIT) {
+      float x = e < n ? static_cast<const float*>(src)[from + e] : 0.0f;
+      if (!(fabsf(x) <= 3.402823466e38f)) bad = true, x = 0.0f;
+      uint16_t a = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+      if ((a & 0x7fffu) == 0x7f80u) --a;   // the largest f32 would round to infinity
+      const float r = x - __uint_as_float(uint32_t(a) << 16);
+      const __nv_bfloat16 b = __float2bfloat16_rn(r);
+      h[e] = a;
+      h[8 + e] = __bfloat16_as_ushort(b);
+      h[16 + e] = __bfloat16_as_ushort(__float2bfloat16_rn(r - __bfloat162float(b)));
+    } else {
+      h[e] = e < n ? static_cast<const uint16_t*>(src)[from + e] : uint16_t(0);
+    }
+  }
+  if (in) {
+    const int64_t plane = rows * per;
+#pragma unroll
+    for (int q = 0; q < (SPLIT ? 3 : 1); ++q) reinterpret_cast<uint4*>(dst)[q * plane + i] = out[q];
+  }
+  if (SPLIT) {
+    const unsigned lanes = __ballot_sync(0xffffffffu, bad), lane = threadIdx.x & 31;
+    if (in && lane % eighths == 0) {
+      const bool mark = (lanes >> lane) & ((1u << eighths) - 1u);
+      odd[row * heads + head] = mark;
+      if (mark) atomicOr(any, 1);
+    }
+  }
 }
+
+int attn_pack(bool split, const void* src, void* dst, int64_t rows, int heads, int D, int DP, int64_t stride, uint8_t* odd, int* any) {
+  const int64_t n = cdiv(rows * heads * (DP / 8), 256);
+  SIMP_REQUIRE(n <= INT_MAX, SIMP_ERR_SHAPE, "attn_prompt: too many rows and heads");
+  if (n == 0) return SIMP_OK;
+  auto kern = split ? attn_pack_kernel<true> : attn_pack_kernel<false>;
+  kern<<<unsigned(n), 256, 0, ctx().stream>>>(src, static_cast<uint16_t*>(dst), rows, heads, D, DP, stride, odd, any);
+  SIMP_LAUNCH_CHECK();
+  return SIMP_OK;
+}
+
+// 16-bit types on the tensor cores: a positive scale (the maximum of the scores is then the maximum of the scaled ones) and
+// rows that TMA can address; others are copied into padded rows first (library scratch).  1: not taken.
 int attn_prompt_tc(const AttnPromptArgs& a, int dtype) {
-  if (dtype == SIMP_DTYPE_BF16) return a.D == 64 ? tc_launch<true, 64>(a) : tc_launch<true, 128>(a);
-  return a.D == 64 ? tc_launch<false, 64>(a) : tc_launch<false, 128>(a);
+  if (dtype == SIMP_DTYPE_F32 || !(a.scale_log2 > 0.0f && a.scale_log2 <= 3.0e38f) || a.total_k == 0) return 1;
+  const int D = a.D <= 64 ? 64 : 128;
+  TcArgs p{};
+  p.a = a;
+  p.whole = a.D == D && aligned_to(a.out, 16) && a.out_stride % 8 == 0;
+  p.q = a.q;
+  p.k = a.k;
+  p.v = a.v;
+  p.q_stride = a.q_stride;
+  p.kv_stride = a.kv_stride;
+  if (a.D != D || !aligned_to(a.q, 16) || !aligned_to(a.k, 16) || !aligned_to(a.v, 16) || a.q_stride % 8 || a.kv_stride % 8) {
+    const size_t nq = size_t(a.total_q) * a.H * D * 2, nk = size_t(a.total_k) * a.G * D * 2;
+    uint8_t* s = static_cast<uint8_t*>(scratch(nq + 2 * nk, SCRATCH_ATTN_PACK));
+    if (!s) return 1;
+    p.q = s;
+    p.k = s + nq;
+    p.v = s + nq + nk;
+    p.q_stride = int64_t(a.H) * D;
+    p.kv_stride = int64_t(a.G) * D;
+    if (int rc = attn_pack(false, a.q, s, a.total_q, a.H, a.D, D, a.q_stride, nullptr, nullptr)) return rc;
+    if (int rc = attn_pack(false, a.k, s + nq, a.total_k, a.G, a.D, D, a.kv_stride, nullptr, nullptr)) return rc;
+    if (int rc = attn_pack(false, a.v, s + nq + nk, a.total_k, a.G, a.D, D, a.kv_stride, nullptr, nullptr)) return rc;
+  }
+  if (dtype == SIMP_DTYPE_BF16) return D == 64 ? tc_launch<true, 64>(p) : tc_launch<true, 128>(p);
+  return D == 64 ? tc_launch<false, 64>(p) : tc_launch<false, 128>(p);
 }
 
 }  // namespace simp

@@ -12,6 +12,8 @@ constexpr int SCRATCH_KV8_PART = 16;   // partial results of a split cache atten
 constexpr int SCRATCH_KV8_COUNT = 17;  // its arrival counters (zero between calls)
 constexpr int SCRATCH_ARGMAX = 18;     // row keys and arrival counters of logits_process (zero between calls)
 
+constexpr int SCRATCH_ATTN_PACK = 19;  // padded or split copies of q, k, v
+
 constexpr int STATUS_BAD_BLOCK = 3, STATUS_BAD_RANGE = 4;
 
 // The calling thread's current device is the library's for the duration of a call (a host thread that never set one
