@@ -8,6 +8,7 @@
 #include <climits>
 
 #include "llm_ops.cuh"
+#include "sm100_ptx.cuh"
 
 namespace simp {
 
@@ -186,6 +187,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8View c, const T* __r
                                                          const int32_t* __restrict__ starts, int n_seqs, int64_t total, int* status) {
   __shared__ float tops[2][8];
   Kv8Span sp;
+  pdl_launch_dependents();
+  pdl_wait();
   if (!kv8_span(c, blockIdx.x, off, starts, n_seqs, total, status, sp)) return;
   const int h = blockIdx.y, quads = c.pitch >> 2, g = threadIdx.x / quads, d = 4 * (threadIdx.x % quads);
   const int t0 = 16 * g, lo = max(sp.a - t0, 0), hi = g < (c.bt >> 4) ? min(sp.b - t0, 16) : 0;   // new tokens of the patch: [lo, hi)
@@ -292,6 +295,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8View c, T* __restrict_
                                                        const int32_t* __restrict__ off, const int32_t* __restrict__ starts,
                                                        int n_seqs, int64_t total, int* status) {
   Kv8Span sp;
+  pdl_launch_dependents();
+  pdl_wait();
   if (!kv8_span(c, blockIdx.x, off, starts, n_seqs, total, status, sp)) return;
   const int h = blockIdx.y, quads = c.pitch >> 2, g = threadIdx.x / quads, d = 4 * (threadIdx.x % quads);
   const int t0 = 16 * g, lo = max(sp.a - t0, 0), hi = g < (c.bt >> 4) ? min(sp.b - t0, 16) : 0;
@@ -322,8 +327,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8View c, T* __restrict_
 }
 
 // ------------------------------------------------------------------------------------------------ attention
-// out = softmax(scale q . K) V for one token per sequence.  Bound by the cache's bytes, so they go from global memory
-// into the MMA operand registers as they are: mma.m16n8k32 with A = 16 tokens x 32 elements of K (s8) and B = the query,
+// out = softmax(scale q . K) V for one token per sequence.  Bound by the cache's bytes, which bulk copies bring into a ring
+// in shared memory and which go from there into the MMA operand registers as they are: mma.m16n8k32 with A = 16 tokens x 32 elements of K (s8) and B = the query,
 // then A = 16 elements x 32 tokens of V (s8) and B = the softmax weights.  Queries and weights become integers of PLANES
 // bytes (16 bits for 16-bit queries, 24 for f32: below the rounding of their own type), one byte plane per B column, so
 // the heads of a group fill the eight columns (4 heads x 2 planes; the third planes of eight heads share one more) and
@@ -340,14 +345,14 @@ struct AttnKv8Args {
   void* out;
   int64_t q_stride, out_stride;
   const int32_t* lengths;
-  float* part;        // [seq][kv head][group][chunk] x (heads x (D + 2))
+  float* part;        // [seq][kv head][group][chunk] x (heads x (pitch + 2))
   int* count;         // [seq][kv head][group]
   int* status;
   float scale_log2;   // scale * log2(e)
   int rep, max_len, chunk, max_chunks, dtype;
 };
 
-constexpr int AK_WARPS = 4;
+constexpr int AK_WARPS = 4, AK_JOIN = 8;
 
 __device__ __forceinline__ void mma_s8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -359,9 +364,9 @@ __device__ __forceinline__ void mma_s8u8(int (&d)[4], uint32_t a0, uint32_t a1, 
                : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint2 ld_stream_u2(const void* p) {
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
 }
 // byte `b` of four integers as one word
@@ -371,22 +376,43 @@ template <int B> __device__ __forceinline__ uint32_t bytes_of(uint32_t x0, uint3
 }
 
 // S = pitch / 32; PLANES = 2 (16-bit queries) or 3 (f32); NH = groups of four heads (1 or 2)
+template <int S>
+struct AttnKv8Ring {
+  // Stages of a tile (K and V of 32 tokens, 64 bytes per element) per warp.  With two of 8 KB, four warps and three blocks
+  // per SM have 96 KB on their way while as much is worked on, about twice what the memory's latency needs.
+  static constexpr int STAGES = S >= 3 ? 2 : 4, STAGE = 64 * 32 * S;
+  static constexpr size_t SMEM = size_t(AK_WARPS) * STAGES * STAGE;
+};
 template <int S, int PLANES, int NH>
 __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Args a) {
-  constexpr int P = 32 * S, HEADS = 4 * NH, NT = NH + (PLANES == 3 ? 1 : 0);
+  constexpr int P = 32 * S, HEADS = 4 * NH, NT = NH + (PLANES == 3 ? 1 : 0), STEP = 32 * AK_WARPS;
+  constexpr int STAGES = AttnKv8Ring<S>::STAGES, STAGE = AttnKv8Ring<S>::STAGE;
   constexpr float QMAX = PLANES == 3 ? 8323072.0f : 32512.0f;      // 127 << 16, 127 << 8: top byte never overflows
   constexpr float PMAX = PLANES == 3 ? 16777215.0f : 65535.0f;
+  extern __shared__ __align__(128) uint8_t ak_ring[];              // [warp][stage][K 32 x P, V 2 x P x 16]; at the end [warp][head][P] sums
   __shared__ __align__(16) int8_t qb[NT * 8][P];                   // byte planes, one row per B column
   __shared__ float qs[HEADS];
   __shared__ float om[AK_WARPS][HEADS], ol[AK_WARPS][HEADS];
-  __shared__ __align__(16) float oacc[AK_WARPS][HEADS][P];
-  __shared__ int last;
+  __shared__ __align__(8) uint64_t bars[AK_WARPS][STAGES];
+  __shared__ int last, abort_flag;
   const Kv8View& c = a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n_groups = (a.rep + HEADS - 1) / HEADS;
   const int s = blockIdx.z, kvh = blockIdx.y / n_groups, hg = blockIdx.y % n_groups, chunk = blockIdx.x;
   const int h0 = kvh * a.rep + hg * HEADS, nh = min(HEADS, a.rep - hg * HEADS);
   const int64_t orow = s * a.out_stride + int64_t(h0) * c.D;
+  const int32_t* table = c.table + s * c.table_stride;
+  const int c0 = chunk * a.chunk, tile0 = c0 + 32 * warp;
+  // Block numbers of a tile's two halves (tokens 0-15, 16-31), the first ones beside the length: a place below max_len has
+  // an entry in the table.  Where the second half lies behind the sequence, the first half's block stands in.
+  auto entries = [&](int tile, int limit, int& e0, int& e1) {
+    e0 = __ldg(table + (tile >> c.shift));
+    e1 = __ldg(table + ((tile + 16 < limit ? tile + 16 : tile) >> c.shift));
+  };
+  int e0 = 0, e1 = 0;
+  pdl_launch_dependents();
+  pdl_wait();
+  if (tile0 < a.max_len) entries(tile0, a.max_len, e0, e1);
   const int len = __ldg(a.lengths + s);
   if (len < 0 || len > a.max_len) {
     if (threadIdx.x == 0) report_status(a.status, STATUS_BAD_RANGE, s);
@@ -397,6 +423,55 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
     if (len == 0 && chunk == 0)
       for (int i = threadIdx.x; i < nh * c.D; i += blockDim.x) store_any(a.out, orow + i, 0.0f, a.dtype);
     return;
+  }
+  const int c1 = min(len, c0 + a.chunk);
+  const int64_t head_bytes = int64_t(c.bt) * P;
+  uint8_t* mine = ak_ring + size_t(warp) * STAGES * STAGE;
+  const uint32_t ring = ptx::smem_u32(mine);
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane == 0)
+    for (int i = 0; i < STAGES; ++i) ptx::mbar_init(ptx::smem_u32(&bars[warp][i]), 1);
+  ptx::fence_barrier_init();
+  __syncwarp();
+  // Requests a tile into a stage; returns this lane's scales (tokens 4 g ..: half g / 4) and whether its block is out of range.
+  struct TileInfo {
+    float ks, vs;
+    bool bad;
+  };
+  auto request = [&](int tile, int stage, int b0, int b1) {
+    const bool bad0 = b0 < 0 || b0 >= c.n_blocks, bad1 = tile + 16 < len && (b1 < 0 || b1 >= c.n_blocks);
+    if (bad0 || bad1) {
+      if (lane == 0) report_status(a.status, STATUS_BAD_BLOCK, bad0 ? b0 : b1);
+    }
+    if (bad0) b0 = 0;
+    if (bad1 || tile + 16 >= len) b1 = b0;
+    const int64_t at0 = int64_t(b0) * c.G + kvh, at1 = int64_t(b1) * c.G + kvh;
+    if (lane == 0) {
+      const uint32_t dst = ring + stage * STAGE, bar = ptx::smem_u32(&bars[warp][stage]);
+      ptx::mbar_arrive_expect_tx(bar, STAGE);
+      const int64_t off = int64_t(tile & (c.bt - 1)) * P;   // K rows and V groups of 16 tokens take the same bytes
+      if (c.bt >= 32) {
+        ptx::bulk_load(dst, c.k + at0 * head_bytes + off, 32 * P, bar);
+        ptx::bulk_load(dst + 32 * P, c.v + at0 * head_bytes + off, 32 * P, bar);
+      } else {
+        ptx::bulk_load(dst, c.k + at0 * head_bytes, 16 * P, bar);
+        ptx::bulk_load(dst + 16 * P, c.k + at1 * head_bytes, 16 * P, bar);
+        ptx::bulk_load(dst + 32 * P, c.v + at0 * head_bytes, 16 * P, bar);
+        ptx::bulk_load(dst + 48 * P, c.v + at1 * head_bytes, 16 * P, bar);
+      }
+    }
+    const int64_t at = g & 4 ? at1 : at0;
+    const bool bad = g & 4 ? bad1 : bad0;
+    return TileInfo{__ldg(c.ks + at), bad ? 0.0f : __ldg(c.vs + at), bad};
+  };
+  TileInfo info[STAGES];
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) {
+    const int tile = tile0 + i * STEP;
+    if (tile < c1) {
+      if (i > 0) entries(tile, len, e0, e1);
+      info[i] = request(tile, i, e0, e1);
+    }
   }
   // ---- the query as byte planes
   for (int h = warp; h < HEADS; h += AK_WARPS) {
@@ -434,13 +509,13 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
     if (lane == 0) qs[h] = odd ? __int_as_float(0x7fc00000) : top / QMAX * a.scale_log2;
   }
   __syncthreads();
-  // B fragments: column g, elements 32 i + 8 t .. + 7 (the contraction order of the K loads below)
+  // B fragments: column g, elements 32 i + 8 t .. + 7 (the contraction order of the K words below)
   uint32_t qf[NT][S][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      // S even: a 16-byte load covers two steps of a 64-element half; S odd: the last 32 elements by 8-byte loads
+      // S even: a 16-byte word covers two steps of a 64-element half; S odd: the last 32 elements by 8-byte words
       const int e = (i < (S & ~1)) ? 64 * (i >> 1) + 16 * t + 8 * (i & 1) : 32 * i + 8 * t;
       const uint2 w = *reinterpret_cast<const uint2*>(&qb[n * 8 + g][e]);
       qf[n][i][0] = w.x;
@@ -460,137 +535,141 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[i][n][r] = 0.0f;
 
-  const int c0 = chunk * a.chunk, c1 = min(len, c0 + a.chunk);
-  const int32_t* table = a.c.table + s * c.table_stride;
-  const int64_t head_bytes = int64_t(c.bt) * P;
-  // block of the 16 tokens from `tok` on; tokens behind the sequence use the block of the tile's first token
-  auto entry = [&](int tile, int half) {
-    const int tok = tile + 16 * half;
-    return __ldg(table + ((tok < len ? tok : tile) >> c.shift));
-  };
-  for (int tile = c0 + 32 * warp; tile < c1; tile += 32 * AK_WARPS) {
-    int be = entry(tile, g >> 2), bv = entry(tile, t >> 1);
-    const bool bad = be < 0 || be >= c.n_blocks;
-    if (bad) report_status(a.status, STATUS_BAD_BLOCK, be), be = 0;
-    if (bv < 0 || bv >= c.n_blocks) bv = 0;
-    const float ks = __ldg(c.ks + int64_t(be) * c.G + kvh), vs = bad ? 0.0f : __ldg(c.vs + int64_t(be) * c.G + kvh);
-    const int8_t* kp = c.k + (int64_t(be) * c.G + kvh) * head_bytes + (((tile + 4 * g) & (c.bt - 1))) * P;
-    const int8_t* vp = c.v + (int64_t(bv) * c.G + kvh) * head_bytes + int64_t(((tile + 8 * t) & (c.bt - 1)) >> 4) * P * 16 + 8 * (t & 1);
-    uint32_t kw[4][2 * S];
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int tile = tile0; ok && tile < c1;) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-#pragma unroll
-      for (int i = 0; i < S / 2; ++i) {
-        const uint4 w = ld_stream_u4(kp + r * P + 64 * i + 16 * t);
-        kw[r][4 * i] = w.x; kw[r][4 * i + 1] = w.y; kw[r][4 * i + 2] = w.z; kw[r][4 * i + 3] = w.w;
+    for (int stage = 0; stage < STAGES; ++stage, tile += STEP) {
+      if (tile >= c1) break;
+      const int next = tile + STAGES * STEP;
+      if (next < c1) entries(next, len, e0, e1);   // arrive while this tile is worked on
+      ok = ptx::mbar_wait(ptx::smem_u32(&bars[warp][stage]), phase, &abort_flag, a.status, 81);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
       }
-      if (S & 1) {
-        const uint2 w = ld_stream_u2(kp + r * P + 32 * (S - 1) + 8 * t);
-        kw[r][2 * S - 2] = w.x; kw[r][2 * S - 1] = w.y;
-      }
-    }
-    uint2 vw[2 * S][2];
+      const uint32_t kp = ring + stage * STAGE + 4 * g * P, vp = ring + stage * STAGE + 32 * P + (t >> 1) * (16 * P) + 8 * (t & 1) + 16 * g;
+      const float k_step = info[stage].ks, v_step = info[stage].vs;
+      const bool masked = info[stage].bad;
+      // ---- scores
+      int acc[2][NT][4];
 #pragma unroll
-    for (int i = 0; i < 2 * S; ++i) {
-      vw[i][0] = ld_stream_u2(vp + (16 * i + g) * 16);
-      vw[i][1] = ld_stream_u2(vp + (16 * i + 8 + g) * 16);
-    }
-    // ---- scores
-    int acc[2][NT][4];
+      for (int mg = 0; mg < 2; ++mg) {
+        uint32_t kw[2][2 * S];
 #pragma unroll
-    for (int mg = 0; mg < 2; ++mg)
+        for (int r = 0; r < 2; ++r) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[mg][n][r] = 0;
-#pragma unroll
-        for (int i = 0; i < S; ++i)
-          mma_s8s8(acc[mg][n], kw[2 * mg][2 * i], kw[2 * mg + 1][2 * i], kw[2 * mg][2 * i + 1], kw[2 * mg + 1][2 * i + 1], qf[n][i][0], qf[n][i][1]);
-      }
-    const float vs_top = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 16));
-    const float vs_rel = vs_top > 0.0f ? vs / vs_top : 0.0f;
-    uint32_t pw[NH][PLANES];
-    float fac[NH];
-#pragma unroll
-    for (int n = 0; n < NH; ++n) {
-      float sc[4], tm = -INFINITY;
-      const float f = hs[n] * ks;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int* x = acc[j >> 1][n] + 2 * (j & 1);
-        float v = float(x[0] * 256 + x[1]);
-        if (PLANES == 3) v = fmaf(v, 256.0f, float(acc[j >> 1][NT - 1][2 * (j & 1) + n]));
-        sc[j] = tile + 4 * g + j < len && !bad ? v * f : -INFINITY;
-        tm = fmaxf(tm, sc[j]);
-      }
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, x));
-      const float mn = fmaxf(m[n], tm);
-      const float alpha = m[n] == -INFINITY ? 0.0f : exp2f(m[n] - mn), beta = tm == -INFINITY ? 0.0f : exp2f(tm - mn);
-      float p[4], sum = 0.0f;
-      uint32_t pi[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        p[j] = sc[j] == -INFINITY ? 0.0f : exp2f(sc[j] - tm);
-        sum += p[j];
-        pi[j] = __float2uint_rn(p[j] * vs_rel * PMAX);
-      }
-      if (__any_sync(0xffffffffu, alpha != 1.0f)) {
-        l[n] *= alpha;
-#pragma unroll
-        for (int i = 0; i < 2 * S; ++i) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[i][n][r] *= alpha;
-          if (PLANES == 3) {
-            o[i][NT - 1][n] *= alpha;
-            o[i][NT - 1][2 + n] *= alpha;
+          for (int i = 0; i < S / 2; ++i) {
+            const uint4 w = ptx::lds128(kp + (2 * mg + r) * P + 64 * i + 16 * t);
+            kw[r][4 * i] = w.x; kw[r][4 * i + 1] = w.y; kw[r][4 * i + 2] = w.z; kw[r][4 * i + 3] = w.w;
+          }
+          if (S & 1) {
+            const uint2 w = lds64(kp + (2 * mg + r) * P + 32 * (S - 1) + 8 * t);
+            kw[r][2 * S - 2] = w.x; kw[r][2 * S - 1] = w.y;
           }
         }
-      }
-      l[n] = fmaf(sum, beta, l[n]);
-      m[n] = mn;
-      fac[n] = beta * vs_top;
-      if (PLANES == 3) {
-        pw[n][0] = bytes_of<2>(pi[0], pi[1], pi[2], pi[3]);
-        pw[n][1] = bytes_of<1>(pi[0], pi[1], pi[2], pi[3]);
-        pw[n][PLANES - 1] = bytes_of<0>(pi[0], pi[1], pi[2], pi[3]);
-      } else {
-        pw[n][0] = bytes_of<1>(pi[0], pi[1], pi[2], pi[3]);
-        pw[n][1] = bytes_of<0>(pi[0], pi[1], pi[2], pi[3]);
-      }
-    }
-    // ---- weights to the B operand: column g = (head g / 2, plane g % 2), tokens 8 t .. 8 t + 7
-    uint32_t pf[NT][2];
-    const int src = 8 * t + (g >> 1);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[mg][n][r] = 0;
+#pragma unroll
+          for (int i = 0; i < S; ++i) mma_s8s8(acc[mg][n], kw[0][2 * i], kw[1][2 * i], kw[0][2 * i + 1], kw[1][2 * i + 1], qf[n][i][0], qf[n][i][1]);
+        }
+      }
+      const float vs_top = fmaxf(v_step, __shfl_xor_sync(0xffffffffu, v_step, 16));
+      const float vs_rel = vs_top > 0.0f ? v_step / vs_top : 0.0f;
+      uint32_t pw[NH][PLANES];
+      float fac[NH];
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
-        const uint32_t hi = __shfl_sync(0xffffffffu, pw[n][0], src + 4 * b), lo = __shfl_sync(0xffffffffu, pw[n][1], src + 4 * b);
-        pf[n][b] = g & 1 ? lo : hi;
+        float sc[4], tm = -INFINITY;
+        const float f = hs[n] * k_step;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int* x = acc[j >> 1][n] + 2 * (j & 1);
+          float v = float(x[0] * 256 + x[1]);
+          if (PLANES == 3) v = fmaf(v, 256.0f, float(acc[j >> 1][NT - 1][2 * (j & 1) + n]));
+          sc[j] = tile + 4 * g + j < len && !masked ? v * f : -INFINITY;
+          tm = fmaxf(tm, sc[j]);
+        }
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, x));
+        const float mn = fmaxf(m[n], tm);
+        const float alpha = m[n] == -INFINITY ? 0.0f : exp2f(m[n] - mn), beta = tm == -INFINITY ? 0.0f : exp2f(tm - mn);
+        float sum = 0.0f;
+        uint32_t pi[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = sc[j] == -INFINITY ? 0.0f : exp2f(sc[j] - tm);
+          sum += p;
+          pi[j] = __float2uint_rn(p * vs_rel * PMAX);
+        }
+        if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+          l[n] *= alpha;
+#pragma unroll
+          for (int i = 0; i < 2 * S; ++i) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[i][n][r] *= alpha;
+            if (PLANES == 3) {
+              o[i][NT - 1][n] *= alpha;
+              o[i][NT - 1][2 + n] *= alpha;
+            }
+          }
+        }
+        l[n] = fmaf(sum, beta, l[n]);
+        m[n] = mn;
+        fac[n] = beta * vs_top;
+        if (PLANES == 3) {
+          pw[n][0] = bytes_of<2>(pi[0], pi[1], pi[2], pi[3]);
+          pw[n][1] = bytes_of<1>(pi[0], pi[1], pi[2], pi[3]);
+          pw[n][PLANES - 1] = bytes_of<0>(pi[0], pi[1], pi[2], pi[3]);
+        } else {
+          pw[n][0] = bytes_of<1>(pi[0], pi[1], pi[2], pi[3]);
+          pw[n][1] = bytes_of<0>(pi[0], pi[1], pi[2], pi[3]);
+        }
       }
-      if (PLANES == 3) {
-        const uint32_t x = __shfl_sync(0xffffffffu, pw[0][PLANES - 1], src + 4 * b);
-        const uint32_t y = NH == 2 ? __shfl_sync(0xffffffffu, pw[NH - 1][PLANES - 1], src + 4 * b) : 0u;
-        pf[NT - 1][b] = g & 1 ? y : x;
+      // ---- weights to the B operand: column g = (head g / 2, plane g % 2), tokens 8 t .. 8 t + 7
+      uint32_t pf[NT][2];
+      const int src = 8 * t + (g >> 1);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+          const uint32_t hi = __shfl_sync(0xffffffffu, pw[n][0], src + 4 * b), lo = __shfl_sync(0xffffffffu, pw[n][1], src + 4 * b);
+          pf[n][b] = g & 1 ? lo : hi;
+        }
+        if (PLANES == 3) {
+          const uint32_t x = __shfl_sync(0xffffffffu, pw[0][PLANES - 1], src + 4 * b);
+          const uint32_t y = NH == 2 ? __shfl_sync(0xffffffffu, pw[NH - 1][PLANES - 1], src + 4 * b) : 0u;
+          pf[NT - 1][b] = g & 1 ? y : x;
+        }
       }
+      // ---- values
+#pragma unroll
+      for (int i = 0; i < 2 * S; ++i) {
+        const uint2 v0 = lds64(vp + 256 * i), v1 = lds64(vp + 256 * i + 128);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          int d[4] = {0, 0, 0, 0};
+          mma_s8u8(d, v0.x, v1.x, v0.y, v1.y, pf[n][0], pf[n][1]);
+          const bool third = PLANES == 3 && n == NT - 1;
+          const float f0 = third ? fac[0] : fac[n < NH ? n : 0], f1 = third ? fac[NH - 1] : f0;
+          o[i][n][0] = fmaf(float(d[0]), f0, o[i][n][0]);
+          o[i][n][1] = fmaf(float(d[1]), f1, o[i][n][1]);
+          o[i][n][2] = fmaf(float(d[2]), f0, o[i][n][2]);
+          o[i][n][3] = fmaf(float(d[3]), f1, o[i][n][3]);
+        }
+      }
+      __syncwarp();   // every lane has read the stage
+      if (next < c1) info[stage] = request(next, stage, e0, e1);
     }
-    // ---- values
-#pragma unroll
-    for (int i = 0; i < 2 * S; ++i)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        int d[4] = {0, 0, 0, 0};
-        mma_s8u8(d, vw[i][0].x, vw[i][1].x, vw[i][0].y, vw[i][1].y, pf[n][0], pf[n][1]);
-        const bool third = PLANES == 3 && n == NT - 1;
-        const float f0 = third ? fac[0] : fac[n < NH ? n : 0], f1 = third ? fac[NH - 1] : f0;
-        o[i][n][0] = fmaf(float(d[0]), f0, o[i][n][0]);
-        o[i][n][1] = fmaf(float(d[1]), f1, o[i][n][1]);
-        o[i][n][2] = fmaf(float(d[2]), f0, o[i][n][2]);
-        o[i][n][3] = fmaf(float(d[3]), f1, o[i][n][3]);
-      }
+    phase ^= 1u;
   }
-  // ---- planes together, warps together
+  if (!ok)
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);   // let copies in flight land
+  // ---- planes together, warps together (the sums take the place of this warp's ring)
+  float(*oacc)[P] = reinterpret_cast<float(*)[P]>(mine);
+  __syncwarp();
 #pragma unroll
   for (int n = 0; n < NH; ++n) {
 #pragma unroll
@@ -606,15 +685,21 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
       for (int r = 0; r < 2; ++r) {
         float v = fmaf(o[i][n][2 * r], 256.0f, o[i][n][2 * r + 1]);
         if (PLANES == 3) v = fmaf(v, 256.0f, o[i][NT - 1][2 * r + n]);
-        oacc[warp][h][16 * i + 8 * r + g] = v * (1.0f / PMAX);
+        oacc[h][16 * i + 8 * r + g] = v * (1.0f / PMAX);
       }
   }
   __syncthreads();
-  const int stride = HEADS * (c.D + 2);
-  const int64_t slot = (int64_t(s) * gridDim.y + blockIdx.y);
-  float* part = a.part + (slot * a.max_chunks + chunk) * stride;
-  for (int i = threadIdx.x; i < nh * c.D; i += blockDim.x) {
-    const int h = i / c.D, d = i - h * c.D;
+  // a part: top and sum of each head, then its P sums; 16-byte aligned
+  constexpr int PART = HEADS * (P + 2);
+  const int64_t slot = int64_t(s) * gridDim.y + blockIdx.y;
+  float* part = a.part + (slot * a.max_chunks + chunk) * PART;
+  auto finish = [&](int h, int d, float val, float den) {   // den is 0 where every block was out of range; NaN stays
+    float r = den > 0.0f ? val / den : den;
+    if (qs[h] != qs[h]) r = qs[h];
+    if (d < c.D) store_any(a.out, orow + h * c.D + d, r, a.dtype);
+  };
+  for (int i = threadIdx.x; i < nh * P; i += blockDim.x) {
+    const int h = i / P, d = i - h * P;
     float top = -INFINITY, den = 0.0f, val = 0.0f;
 #pragma unroll
     for (int w = 0; w < AK_WARPS; ++w) top = fmaxf(top, om[w][h]);
@@ -622,14 +707,12 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
     for (int w = 0; w < AK_WARPS; ++w) {
       const float f = om[w][h] == -INFINITY ? 0.0f : exp2f(om[w][h] - top);
       den = fmaf(ol[w][h], f, den);
-      val = fmaf(oacc[w][h][d], f, val);
+      val = fmaf(reinterpret_cast<const float*>(ak_ring + size_t(w) * STAGES * STAGE)[h * P + d], f, val);
     }
     if (n_chunks == 1) {
-      float r = den > 0.0f ? val / den : den;   // den is 0 where every block was out of range; NaN stays
-      if (qs[h] != qs[h]) r = qs[h];
-      store_any(a.out, orow + i, r, a.dtype);
+      finish(h, d, val, den);
     } else {
-      part[2 * HEADS + h * c.D + d] = val;
+      part[2 * HEADS + i] = val;
       if (d == 0) {
         part[2 * h] = top;
         part[2 * h + 1] = den;
@@ -644,29 +727,49 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
   __syncthreads();
   if (!last) return;
   __threadfence();
-  const float* all = a.part + slot * a.max_chunks * stride;
-  for (int i = threadIdx.x; i < nh * c.D; i += blockDim.x) {
-    const int h = i / c.D, d = i - h * c.D;
-    float top = -INFINITY, den = 0.0f, val = 0.0f;
-    for (int x = 0; x < n_chunks; ++x) top = fmaxf(top, __ldcg(all + int64_t(x) * stride + 2 * h));
-    for (int x = 0; x < n_chunks; ++x) {
-      const float* p = all + int64_t(x) * stride;
-      const float mx = __ldcg(p + 2 * h), f = mx == -INFINITY ? 0.0f : exp2f(mx - top);
-      den = fmaf(__ldcg(p + 2 * h + 1), f, den);
-      val = fmaf(__ldcg(p + 2 * HEADS + h * c.D + d), f, val);
+  const float* all = a.part + slot * a.max_chunks * PART;
+  for (int i = 4 * threadIdx.x; i < nh * P; i += 4 * blockDim.x) {
+    const int h = i / P, d = i - h * P;
+    float top = -INFINITY, den = 0.0f;
+    float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int x0 = 0; x0 < n_chunks; x0 += AK_JOIN) {   // eight parts are requested together, their sum keeps its order
+      float2 md[AK_JOIN];
+      float4 v[AK_JOIN];
+#pragma unroll
+      for (int x = 0; x < AK_JOIN; ++x) {
+        const float* p = all + int64_t(min(x0 + x, n_chunks - 1)) * PART;
+        md[x] = __ldcg(reinterpret_cast<const float2*>(p + 2 * h));
+        v[x] = __ldcg(reinterpret_cast<const float4*>(p + 2 * HEADS + i));
+        if (x0 + x >= n_chunks) md[x].x = -INFINITY;
+      }
+      float now = top;
+#pragma unroll
+      for (int x = 0; x < AK_JOIN; ++x) now = fmaxf(now, md[x].x);
+      const float keep = top == -INFINITY ? 0.0f : exp2f(top - now);
+      den *= keep;
+      val = make_float4(val.x * keep, val.y * keep, val.z * keep, val.w * keep);
+      top = now;
+#pragma unroll
+      for (int x = 0; x < AK_JOIN; ++x) {
+        const float f = md[x].x == -INFINITY ? 0.0f : exp2f(md[x].x - top);
+        den = fmaf(md[x].y, f, den);
+        val = make_float4(fmaf(v[x].x, f, val.x), fmaf(v[x].y, f, val.y), fmaf(v[x].z, f, val.z), fmaf(v[x].w, f, val.w));
+      }
     }
-    float r = den > 0.0f ? val / den : den;
-    if (qs[h] != qs[h]) r = qs[h];
-    store_any(a.out, orow + i, r, a.dtype);
+    finish(h, d, val.x, den);
+    finish(h, d + 1, val.y, den);
+    finish(h, d + 2, val.z, den);
+    finish(h, d + 3, val.w, den);
   }
   if (threadIdx.x == 0) a.count[slot] = 0;
 }
 
 template <int S, int PLANES>
 static cudaError_t attn_kv8_launch(int nh, dim3 grid, cudaStream_t st, const AttnKv8Args& a) {
-  if (nh == 1) attn_kv8_kernel<S, PLANES, 1><<<grid, AK_WARPS * 32, 0, st>>>(a);
-  else attn_kv8_kernel<S, PLANES, 2><<<grid, AK_WARPS * 32, 0, st>>>(a);
-  return cudaGetLastError();
+  auto kern = nh == 1 ? attn_kv8_kernel<S, PLANES, 1> : attn_kv8_kernel<S, PLANES, 2>;
+  constexpr size_t smem = AttnKv8Ring<S>::SMEM;
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)); e != cudaSuccess) return e;
+  return launch_kernel(kern, grid, dim3(AK_WARPS * 32), smem, st, true, a);
 }
 
 // ------------------------------------------------------------------------------------------------ arguments
@@ -707,20 +810,21 @@ static int kv8_rows(const char* who, bool write, const simp_kv8_cache* cache, co
   const unsigned threads = unsigned((c.bt / 16 * (c.pitch / 4) + 31) / 32 * 32);
   const size_t four = 4 * dtype_size(dtype);
   const bool vec = c.D % 4 == 0 && kv_stride % 4 == 0 && aligned_to(k, four) && aligned_to(v, four);
+  cudaError_t e = cudaSuccess;
   auto go = [&](auto zero) {
     using T = decltype(zero);
     if (write) {
       auto kern = vec ? kv8_append_kernel<T, true> : kv8_append_kernel<T, false>;
-      kern<<<grid, threads, 0, st>>>(c, static_cast<const T*>(k), static_cast<const T*>(v), kv_stride, off, starts, int(n_seqs), total, status);
+      e = launch_kernel(kern, grid, dim3(threads), 0, st, true, c, static_cast<const T*>(k), static_cast<const T*>(v), kv_stride, off, starts, int(n_seqs), total, status);
     } else {
       auto kern = vec ? kv8_read_kernel<T, true> : kv8_read_kernel<T, false>;
-      kern<<<grid, threads, 0, st>>>(c, static_cast<T*>(k), static_cast<T*>(v), kv_stride, off, starts, int(n_seqs), total, status);
+      e = launch_kernel(kern, grid, dim3(threads), 0, st, true, c, static_cast<T*>(k), static_cast<T*>(v), kv_stride, off, starts, int(n_seqs), total, status);
     }
   };
   if (dtype == SIMP_DTYPE_F32) go(float());
   else if (dtype == SIMP_DTYPE_F16) go(__half());
   else go(__nv_bfloat16());
-  SIMP_LAUNCH_CHECK();
+  SIMP_REQUIRE(e == cudaSuccess, SIMP_ERR_CUDA, "%s launch failed: %s", who, cudaGetErrorString(e));
   return SIMP_OK;
 }
 
@@ -776,12 +880,16 @@ SIMP_API int simp_gpu_attn_kv8(const simp_kv8_cache* cache, const int32_t* block
   const int nh = a.rep > 4 ? 2 : 1;
   const int64_t groups = int64_t(a.c.G) * ((a.rep + 4 * nh - 1) / (4 * nh));
   const int64_t slots = n_seqs * groups;
-  // chunks of at least one tile per warp, so many that the SMs have about three blocks each
-  const int64_t least = 32 * AK_WARPS, want = std::max<int64_t>(1, 3 * int64_t(ctx().sm_count) / slots);
+  // Chunks of at least a tile per warp.  One sequence: as many blocks as run at once (three per SM), for joining costs as
+  // much as it gains beyond that (131072 tokens, 8 x 128: 56 us with 54 chunks, 67 with 109, 87 with 205).  Several, whose
+  // lengths differ: twice as many and none longer than 2048 tokens, so that the longest does not end alone (64 sequences of
+  // up to 8097: 126 us, 135 in one chunk each, 131 with 1024).
+  const int64_t least = 32 * AK_WARPS, waves = n_seqs == 1 ? 3 : 6, want = std::max<int64_t>(1, waves * int64_t(ctx().sm_count) / slots);
   a.chunk = int(std::max(least, cdiv(cdiv(std::max<int64_t>(max_len, 1), want), least) * least));
+  if (n_seqs > 1) a.chunk = std::min(a.chunk, 2048);
   a.max_chunks = int(std::max<int64_t>(1, cdiv(max_len, a.chunk)));
   if (a.max_chunks > 1) {
-    a.part = static_cast<float*>(scratch(size_t(slots) * a.max_chunks * 4 * nh * (a.c.D + 2) * 4, SCRATCH_KV8_PART));
+    a.part = static_cast<float*>(scratch(size_t(slots) * a.max_chunks * 4 * nh * (a.c.pitch + 2) * 4, SCRATCH_KV8_PART));
     if (!a.part) return scratch_failed("attn_kv8");
     a.count = static_cast<int*>(scratch(size_t(slots) * 4, SCRATCH_KV8_COUNT, true));
     if (!a.count) return scratch_failed("attn_kv8");

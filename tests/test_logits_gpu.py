@@ -204,3 +204,16 @@ def test_recorded(gpu):
     want = torch.from_numpy(expected(c))
     assert equal(back(gpu, bo, c["x"]), want) and np.array_equal(best.to_numpy(np.int32, 20), greedy(want))
     rec.close()
+
+
+@pytest.mark.parametrize("rows,vocab,biases", [(1, 9000, 20000), (40, 128256, 9000)])
+def test_long_lists(gpu, rows, vocab, biases):
+    """More biases than the usual path takes, many for the same token; histories longer than a thread keeps at hand."""
+    c = make(11, rows, vocab, "f32", 6000, 10, "rows")
+    rng = np.random.default_rng(12)
+    c["nb"] = [biases - 7 * r for r in range(rows)]
+    c["bid"] = rng.integers(0, vocab, sum(c["nb"])).astype(np.int32)
+    c["bval"] = rng.standard_normal(sum(c["nb"])).astype(np.float32)
+    want = torch.from_numpy(expected(c))
+    out, best = run(gpu, c)
+    assert equal(out, want) and np.array_equal(best, greedy(want))
