@@ -30,7 +30,7 @@ template <int D>
 struct F3Shape {
   static constexpr int QPLANE = 128 * D * 2, KPLANE = F3_KEYS * D * 2;
   static constexpr int BARS = 9;
-  static constexpr size_t SMEM = 3 * size_t(QPLANE) + 6 * size_t(KPLANE) + BARS * 8 + 16 + 8 * 128;
+  static constexpr size_t SMEM = 3 * size_t(QPLANE) + 6 * size_t(KPLANE) + BARS * 8 + 16 + 8 * 128 + 24;
   static constexpr uint32_t TMEM = D == 64 ? 256 : 512, P = 64, T = D == 64 ? 160 : 256;   // columns: S at 0, three P planes, T
 };
 static_assert(F3Shape<128>::SMEM <= 232448 && 2 * F3Shape<64>::SMEM <= 228 * 1024 - 2048, "");
@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8);
   float* half_row = reinterpret_cast<float*>(tail + 16);   // [half][row]
+  volatile int* found_unit = reinterpret_cast<volatile int*>(half_row + 2 * 128);   // found, place, q0, q1, k0, k1
   const AttnPromptArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {   // never: the declaration asks for it
@@ -81,22 +82,32 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
     *abort_flag = 0;
     fence_barrier_init();
   }
-  // ---- which rows
+  pdl_launch_dependents();
+  pdl_wait();
+  // ---- which rows: found by one warp while the others prepare
   const int g = blockIdx.x % a.G;
-  int seq = 0, place = 0, q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-  auto count = [&](int s) {
-    int b, e;
-    return seq_range(a.q_off, s, a.total_q, a.status, b, e) ? (e - b + p.tpt - 1) / p.tpt : 0;
-  };
-  if (!find_unit(blockIdx.x / a.G, a.n_seqs, count, seq, place)) return;
-  seq_range(a.q_off, seq, a.total_q, a.status, q0, q1);
-  if (!seq_range(a.k_off, seq, a.total_k, a.status, k0, k1)) return;
-  const int nq = q1 - q0, nk = k1 - k0;
-  const int r0 = ((nq + p.tpt - 1) / p.tpt - 1 - place) * p.tpt;   // the longest rows first
-  const int64_t shift = int64_t(nk) - nq;
-  auto sees = [&](int token) { return int(max(int64_t(0), min(int64_t(nk), token + shift + 1))); };
-  const int n = (sees(min(r0 + p.tpt, nq) - 1) + F3_KEYS - 1) / F3_KEYS;
-
+  int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+  if (warp == 0) {
+    auto count = [&](int s) {
+      int b, e;
+      return seq_range(a.q_off, s, a.total_q, a.status, b, e) ? (e - b + p.tpt - 1) / p.tpt : 0;
+    };
+    auto keys_of = [&](int s) { return __ldg(a.k_off + s + 1) - __ldg(a.k_off + s); };
+    int seq = 0, place = 0;
+    bool found = find_unit(blockIdx.x / a.G, a.n_seqs, count, seq, place, keys_of);
+    if (found) {
+      seq_range(a.q_off, seq, a.total_q, a.status, q0, q1);
+      found = seq_range(a.k_off, seq, a.total_k, a.status, k0, k1);
+    }
+    if (lane == 0) {
+      found_unit[0] = found;
+      found_unit[1] = place;
+      found_unit[2] = q0;
+      found_unit[3] = q1;
+      found_unit[4] = k0;
+      found_unit[5] = k1;
+    }
+  }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), Sh::TMEM);
     tmem_relinquish();
@@ -105,6 +116,20 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
+  if (!found_unit[0]) {
+    if (warp == 1) tmem_dealloc(tmem, Sh::TMEM);
+    return;
+  }
+  q0 = found_unit[2];
+  q1 = found_unit[3];
+  k0 = found_unit[4];
+  k1 = found_unit[5];
+  const int place = found_unit[1];
+  const int nq = q1 - q0, nk = k1 - k0;
+  const int r0 = ((nq + p.tpt - 1) / p.tpt - 1 - place) * p.tpt;   // the longest rows first
+  const int64_t shift = int64_t(nk) - nq;
+  auto sees = [&](int token) { return int(max(int64_t(0), min(int64_t(nk), token + shift + 1))); };
+  const int n = (sees(min(r0 + p.tpt, nq) - 1) + F3_KEYS - 1) / F3_KEYS;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ loads
@@ -355,8 +380,7 @@ static int f3_launch(F3Args p, const uint8_t* q, const uint8_t* k, const uint8_t
   SIMP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(F3Shape<D>::SMEM)));
   const int64_t units = std::min(a.total_q, a.total_q / p.tpt + a.n_seqs) * a.G;
   SIMP_REQUIRE(units <= INT_MAX, SIMP_ERR_SHAPE, "attn_prompt: too many rows and heads");
-  kern<<<unsigned(units), F3_THREADS, F3Shape<D>::SMEM, ctx().stream>>>(mq, mk, mv, p);
-  SIMP_LAUNCH_CHECK();
+  SIMP_CUDA(launch_kernel(kern, dim3(unsigned(units)), dim3(F3_THREADS), F3Shape<D>::SMEM, ctx().stream, true, mq, mk, mv, p));
   return SIMP_OK;
 }
 

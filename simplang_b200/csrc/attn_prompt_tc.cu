@@ -1,13 +1,13 @@
 // attn_prompt_tc.cu -- causal attention over packed prompts on the tcgen05 tensor cores: f16 / bf16, head size 64 or 128.
 //
-// One block of 20 warps works on two row tiles ("A" and "B") of one key/value head of one sequence.  A row tile is 128 rows
+// One block works on two row tiles ("A" and "B"; short prompts: one) of one key/value head of one sequence.  A row tile is 128 rows
 // of the score matrix: 128 / rep consecutive tokens times the rep query heads that share the key/value head (row = token *
 // rep + head), so grouped heads read K and V once, short prompts fill tiles and the causal edge is fine.  Roles:
-//   warps 0-7, 8-15 softmax of tile A, of tile B: two threads per row, 64 keys each, which exchange their maxima
-//   warp 16         TMA: Q once, then K and V tiles of 128 keys through a ring of slots
-//   warps 17, 19    issue the MMAs of tile A, of tile B: S = Q K^T (128 x 128, f32 in TMEM), O += P V with P read from TMEM.
+//   warp 0          TMA: Q once, then K and V tiles of 128 keys through a ring of slots
+//   warps 1, 2      issue the MMAs of tile A, of tile B: S = Q K^T (128 x 128, f32 in TMEM), O += P V with P read from TMEM.
 //                   Issuing blocks while the tensor cores are busy, so one thread for both would leave them idle at its waits
-//   warp 18         cleans the V tiles at the causal / ragged edge (see below)
+//   warp 3          cleans the V tiles at the causal / ragged edge (see below)
+//   warps 4-11, 12-19  softmax of tile A, of tile B: two threads per row, 64 keys each, which exchange their maxima
 // P (16 bits) overwrites S in place: S_X(j + 1) is issued behind O_X += P_X(j) V(j) by the same thread, whose MMAs run in order.
 // While the tensor cores work on one tile, the other tile's softmax runs: 2 x 128 x 128 x D MACs take 4 D cycles per tile and
 // step, its 16384 exponentials 1024, so for D = 128 both are busy about half of the time.
@@ -18,7 +18,7 @@
 //
 // A weight of zero does not hide a NaN or an infinity from an MMA, and a tile may hold keys that some rows must not see:
 // later tokens of the sequence, and rows of the NEXT sequence (or behind the last) where the sequence ends inside the tile.
-// Warp 18 therefore zeroes, in the edge tiles only, V rows behind the sequence and every element that is not finite; a bit
+// Warp 3 therefore zeroes, in the edge tiles only, V rows behind the sequence and every element that is not finite; a bit
 // per such key tells the epilogue to add those elements (read again from global memory) to the rows that do see the key.
 #include <algorithm>
 #include <climits>
@@ -28,20 +28,33 @@
 
 namespace simp {
 
-constexpr int TC_THREADS = 640;
 constexpr int W_LOAD = 0, W_MMA = 1, W_EDGE = 3;   // W_MMA: tile A, W_MMA + 1: tile B; 4 .. 19: softmax
 constexpr int TC_EDGE = 4;   // edge tiles of a block: its rows see at most 255 keys more than its first row, so 3
 
-template <int D>
-struct TcShape {
-  static constexpr int TILE = 128 * D * 2;              // bytes of 128 rows
-  static constexpr int SLOTS = D == 128 ? 5 : 8;
-  static constexpr int BARS = 2 * SLOTS + 1 + 6 + TC_EDGE;
-  // (1 KB of the 228 belongs to the system: 232448 bytes are a block's most)
-  static constexpr size_t SMEM = size_t(2 + SLOTS) * TILE + BARS * 8 + 16 + TC_EDGE * 16 + 4 * 128 * 4;
-};
+// whether one of eight 16-bit elements is infinity or NaN: one more in the exponent then reaches the sign's place
+template <bool BF16>
+__device__ __forceinline__ bool any_odd(const uint4& w) {
+  constexpr uint32_t E = BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = BF16 ? 0x00800080u : 0x04000400u;
+  return ((((w.x & E) + ONE) | ((w.y & E) + ONE) | ((w.z & E) + ONE) | ((w.w & E) + ONE)) & 0x80008000u) != 0;
+}
+template <bool BF16>
+__device__ __forceinline__ float to_16(uint16_t v) {
+  return BF16 ? __uint_as_float(uint32_t(v) << 16) : __half2float(__ushort_as_half(v));
+}
 
-static_assert(TcShape<128>::SMEM <= 232448 && TcShape<64>::SMEM <= 232448, "");
+// TILES = 2: one block per SM, whose tiles take turns on the tensor cores.  TILES = 1: two blocks per SM, so that one works
+// while the other starts, loads its first tiles or writes its output.
+template <int D, int TILES>
+struct TcShape {
+  static constexpr int THREADS = 128 + 256 * TILES;
+  static constexpr int TILE = 128 * D * 2;              // bytes of 128 rows
+  static constexpr int SLOTS = TILES == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 4);
+  static constexpr int BARS = 2 * SLOTS + 1 + 6 + TC_EDGE;
+  static constexpr uint32_t TMEM = TILES == 2 ? 512 : 256, O = 128 * TILES;   // columns: S of each tile, then O of each
+  // (1 KB of the SM's 228 belongs to the system for each block)
+  static constexpr size_t SMEM = size_t(TILES + SLOTS) * TILE + BARS * 8 + 16 + TC_EDGE * 16 + 2 * TILES * 128 * 4 + 24;
+  static_assert((3 - TILES) * (SMEM + 1024) <= 228 * 1024, "");
+};
 
 struct TcArgs {
   AttnPromptArgs a;
@@ -60,14 +73,14 @@ __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
   return ((w & E) == E ? 0xffffu : 0u) | ((w & (E << 16)) == (E << 16) ? 0xffff0000u : 0u);
 }
 
-template <bool BF16, int D>
-__global__ void __launch_bounds__(TC_THREADS, 1)
+template <bool BF16, int D, int TILES>
+__global__ void __launch_bounds__(128 + 256 * TILES, 3 - TILES)
     attn_prompt_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                           const __grid_constant__ CUtensorMap map_v, const TcArgs p) {
-  using Sh = TcShape<D>;
+  using Sh = TcShape<D, TILES>;
   extern __shared__ __align__(1024) uint8_t tc_raw[];   // swizzled tiles start on 1 KB boundaries
   const uint32_t base = smem_u32(tc_raw);
-  const uint32_t q_smem = base, ring = base + 2 * Sh::TILE, bars = ring + Sh::SLOTS * Sh::TILE;
+  const uint32_t q_smem = base, ring = base + TILES * Sh::TILE, bars = ring + Sh::SLOTS * Sh::TILE;
   uint8_t* generic = tc_raw;
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (Sh::SLOTS + s); };
@@ -81,6 +94,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8);
   uint32_t* odd_keys = reinterpret_cast<uint32_t*>(tail + 16);   // [TC_EDGE][4]: keys of edge tiles with an element that is not finite
   float* half_row = reinterpret_cast<float*>(tail + 16 + TC_EDGE * 16);   // [tile][half][row]: what the two threads of a row exchange
+  volatile int* found_unit = reinterpret_cast<volatile int*>(half_row + 2 * TILES * 128);   // found, place, q0, q1, k0, k1
   const AttnPromptArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {   // never: the declaration asks for it
@@ -91,7 +105,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < Sh::SLOTS; ++s) {
       mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 2);
+      mbar_init(empty_bar(s), TILES);
     }
     mbar_init(q_bar, 1);
     for (int x = 0; x < 2; ++x) {
@@ -105,17 +119,50 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   }
   if (threadIdx.x < TC_EDGE * 4) odd_keys[threadIdx.x] = 0;
 
-  // ---- which rows (every warp finds them for itself)
+  pdl_launch_dependents();
+  pdl_wait();
+  // ---- which rows: found by one warp while the others prepare
   const int g = blockIdx.x % a.G;
-  const int rows_cta = 2 * p.tpt;
-  int seq = 0, place = 0, q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-  auto count = [&](int s) {
-    int b, e;
-    return seq_range(a.q_off, s, a.total_q, a.status, b, e) ? (e - b + rows_cta - 1) / rows_cta : 0;
-  };
-  if (!find_unit(blockIdx.x / a.G, a.n_seqs, count, seq, place)) return;
-  seq_range(a.q_off, seq, a.total_q, a.status, q0, q1);
-  if (!seq_range(a.k_off, seq, a.total_k, a.status, k0, k1)) return;
+  const int rows_cta = TILES * p.tpt;
+  int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+  if (warp == W_LOAD) {
+    auto count = [&](int s) {
+      int b, e;
+      return seq_range(a.q_off, s, a.total_q, a.status, b, e) ? (e - b + rows_cta - 1) / rows_cta : 0;
+    };
+    auto keys_of = [&](int s) { return __ldg(a.k_off + s + 1) - __ldg(a.k_off + s); };
+    int seq = 0, place = 0;
+    bool found = find_unit(blockIdx.x / a.G, a.n_seqs, count, seq, place, keys_of);
+    if (found) {
+      seq_range(a.q_off, seq, a.total_q, a.status, q0, q1);
+      found = seq_range(a.k_off, seq, a.total_k, a.status, k0, k1);
+    }
+    if (lane == 0) {
+      found_unit[0] = found;
+      found_unit[1] = place;
+      found_unit[2] = q0;
+      found_unit[3] = q1;
+      found_unit[4] = k0;
+      found_unit[5] = k1;
+    }
+  }
+  if (warp == W_MMA) {
+    tmem_alloc(smem_u32(tmem_slot), Sh::TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = TILES == 2 ? 0u : *tmem_slot;   // a block that allocates every column starts at 0
+  if (!found_unit[0]) {
+    if (warp == W_MMA) tmem_dealloc(tmem, Sh::TMEM);
+    return;
+  }
+  q0 = found_unit[2];
+  q1 = found_unit[3];
+  k0 = found_unit[4];
+  k1 = found_unit[5];
+  int place = found_unit[1];
   const int nq = q1 - q0, nk = k1 - k0;
   place = (nq + rows_cta - 1) / rows_cta - 1 - place;   // the longest rows first
   const int r0 = place * rows_cta;                      // first token of tile A
@@ -125,23 +172,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const int first = r0 + x * p.tpt, last = min(first + p.tpt, nq) - 1;
-    n_x[x] = first < nq ? (sees(last) + 127) >> 7 : 0;
+    n_x[x] = x < TILES && first < nq ? (sees(last) + 127) >> 7 : 0;
   }
   const int n = max(n_x[0], n_x[1]);
   const int edge0 = sees(r0) >> 7;                      // tiles from here on hold a key that some row does not see
 
-  if (warp == W_MMA) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
-    tmem_relinquish();
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;   // 0: the block allocates every column
-
   // ------------------------------------------------------------------ MMAs of tile X
-  // The whole warp runs this code with the same values and one lane issues; x, the TMEM columns (all 512 are this block's,
-  // so they start at 0) and the descriptors' bases are constants.  Operands of an MMA then live in uniform registers; from
+  // The whole warp runs this code with the same values and one lane issues; x, the TMEM columns (of a block that has all 512)
+  // and the descriptors' bases are constants.  Operands of an MMA then live in uniform registers; from
   // general ones each costs several more instructions, and the warp shares its scheduler with the softmax of the other
   // tile, which leaves few slots (beside warps that issue nothing but FFMA an MMA took 113-130 cycles instead of 64).
   auto mma_role = [&](auto which) {
@@ -158,7 +196,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       if (leader) mma_commit(bar);
     };
     constexpr uint32_t idesc_s = idesc_f16(BF16, 128, false), idesc_o = idesc_f16(BF16, D, true);
-    constexpr uint32_t s_tmem = 128u * x, o_tmem = 256u + uint32_t(D) * x;
+    const uint32_t s_tmem = tmem + 128u * x, o_tmem = tmem + Sh::O + uint32_t(D) * x;
     const uint64_t qd = make_smem_desc_sw128(q_smem + x * Sh::TILE, 16u, 1024u);
     const uint64_t ring_k = make_smem_desc_sw128(ring, 16u, 1024u);
     // V [key][element]: element-major operand, 64-element atoms 16 KB apart, 8 keys 1 KB apart
@@ -232,7 +270,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if (warp == W_LOAD) {
     // ------------------------------------------------------------------ loads
     if (lane == 0 && n > 0) {
-      const int tiles = r0 + p.tpt < nq ? 2 : 1;
+      const int tiles = TILES == 2 && r0 + p.tpt < nq ? 2 : 1;
       const uint32_t box = uint32_t(p.tpt * a.rep) * 128u;
       mbar_arrive_expect_tx(q_bar, tiles * (D / 64) * box);
       for (int x = 0; x < tiles; ++x)
@@ -242,7 +280,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (int i = 0; ok && i < 2 * n; ++i) {
         const int s = i % Sh::SLOTS;
         if (!wait_bar(empty_bar(s), ((i / Sh::SLOTS) & 1) ^ 1, abort_flag, a.status, 61)) { ok = false; break; }
-        const bool edge = (i & 1) && (i >> 1) >= edge0;   // lands for warp 18, which passes the slot on
+        const bool edge = (i & 1) && (i >> 1) >= edge0;   // lands for warp 3, which passes the slot on
         const uint32_t bar = edge ? edge_bar((i >> 1) - edge0) : full_bar(s);
         mbar_arrive_expect_tx(bar, Sh::TILE);
         for (int b = 0; b < D / 64; ++b)
@@ -255,25 +293,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   } else if (warp == W_MMA) {
     mma_role(std::integral_constant<int, 0>());
   } else if (warp == W_MMA + 1) {
-    mma_role(std::integral_constant<int, 1>());
+    if (TILES == 2) mma_role(std::integral_constant<int, 1>());
   } else if (warp == W_EDGE) {
     // ------------------------------------------------------------------ V at the edge
     for (int j = edge0; j < n; ++j) {
       const int i = 2 * j + 1;
       if (!wait_bar(edge_bar(j - edge0), 0, abort_flag, a.status, 66)) break;
-      uint8_t* v = generic + 2 * Sh::TILE + (i % Sh::SLOTS) * Sh::TILE;
-      const int keys = nk - 128 * j;   // rows from here on are not the sequence's
+      uint8_t* v = generic + TILES * Sh::TILE + (i % Sh::SLOTS) * Sh::TILE;
+      const int keys = min(nk - 128 * j, 128);          // rows from here on are not the sequence's
+      const int all_see = max(sees(r0) - 128 * j, 0);   // every row sees the keys before: nothing to hide
       // (the 128-byte swizzle moves 16-byte pieces inside a row only, so rows are found as if there were none)
-      for (int c = lane; c < Sh::TILE / 16; c += 32) {
-        const int key = (c >> 3) & 127;
-        uint4* at = reinterpret_cast<uint4*>(v) + c;
-        uint4 w = *at;
-        uint32_t m0 = odd_halves<BF16>(w.x), m1 = odd_halves<BF16>(w.y), m2 = odd_halves<BF16>(w.z), m3 = odd_halves<BF16>(w.w);
-        if (key >= keys) {
-          *at = make_uint4(0u, 0u, 0u, 0u);
-        } else if (m0 | m1 | m2 | m3) {
-          *at = make_uint4(w.x & ~m0, w.y & ~m1, w.z & ~m2, w.w & ~m3);
-          atomicOr(odd_keys + (j - edge0) * 4 + (key >> 5), 1u << (key & 31));
+#pragma unroll 1
+      for (int b = 0; b < D / 64; ++b) {
+        uint4* atom = reinterpret_cast<uint4*>(v + b * 16384);
+#pragma unroll 1
+        for (int c = 8 * keys + lane; c < 1024; c += 32) atom[c] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+        for (int c0 = 8 * all_see; c0 < 8 * keys; c0 += 256) {
+          uint4 w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = c0 + 32 * e + lane < 8 * keys ? atom[c0 + 32 * e + lane] : make_uint4(0u, 0u, 0u, 0u);
+          uint32_t found = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) found |= any_odd<BF16>(w[e]) ? 1u << e : 0u;
+          if (found)
+#pragma unroll 1
+            for (int e = 0; e < 8; ++e) {
+              if (!((found >> e) & 1u)) continue;
+              const int c = c0 + 32 * e + lane, key = c >> 3;
+              const uint4 o = atom[c];
+              atom[c] = make_uint4(o.x & ~odd_halves<BF16>(o.x), o.y & ~odd_halves<BF16>(o.y), o.z & ~odd_halves<BF16>(o.z), o.w & ~odd_halves<BF16>(o.w));
+              atomicOr(odd_keys + (j - edge0) * 4 + (key >> 5), 1u << (key & 31));
+            }
         }
       }
       fence_proxy_async_smem();
@@ -284,7 +335,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     // ------------------------------------------------------------------ softmax
     const int x = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, row = threadIdx.x & 127;
     const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-    const uint32_t s_tmem = tmem + 128u * x + lanes, o_tmem = tmem + 256u + uint32_t(D) * x + uint32_t(D / 2) * half + lanes;
+    const uint32_t s_tmem = tmem + 128u * x + lanes, o_tmem = tmem + Sh::O + uint32_t(D) * x + uint32_t(D / 2) * half + lanes;
     const int token = r0 + x * p.tpt + row / a.rep, head = g * a.rep + row % a.rep;
     const bool mine = row < p.tpt * a.rep && token < nq;
     const int lim = mine ? sees(token) : 0;
@@ -299,10 +350,32 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       tc_fence_after_sync();
       const int see = lim - 128 * j - 64 * half;
       const bool masked = __any_sync(0xffffffffu, see < 64);
+      const int most = masked ? __reduce_max_sync(0xffffffffu, see) : 64;   // keys behind it no row of the warp sees
       // Weights relative to the maximum so far, and this tile's maximum beside them: the maximum nearly always stays, so the
-      // exponentials need not wait for it.  Where it moves (the first tile always), once more with the new one; S is still
-      // there, P is not stored before the row's two threads agree.
-      for (int attempt = 0;; ++attempt) {
+      // exponentials need not wait for it.  Where it moves, once more with the new one; S is still there, P is not stored before
+      // the row's two threads agree.
+      for (int attempt = j == 0 ? -1 : 0;; attempt = 1) {
+        if (attempt < 0) {   // the first tile: nothing to go by, so its maximum first
+          float t[2] = {-INFINITY, -INFINITY};
+          uint32_t s[2][16];
+          tmem_ld_32x16(s_tmem + 64u * half, s[0]);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            tmem_ld_wait();
+            if (h < 3) tmem_ld_32x16(s_tmem + 64u * half + 16u * (h + 1), s[(h + 1) & 1]);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float s0 = 16 * h + i < see ? __uint_as_float(s[h & 1][i]) : -INFINITY, s1 = 16 * h + i + 1 < see ? __uint_as_float(s[h & 1][i + 1]) : -INFINITY;
+              t[h & 1] = max3(t[h & 1], s0, s1);
+            }
+          }
+          const float top = fmaxf(t[0], t[1]);
+          *to = top;
+          ok = all_of(1 + 4 * x + (warp & 3), 64, ok);
+          if (!ok) break;
+          m = fmaxf(top, *from) * c;
+          continue;
+        }
         const float off = m == -INFINITY ? 0.0f : m;
         const f2 off2 = pack_f2(-off, -off);
         float t[2] = {-INFINITY, -INFINITY};
@@ -313,6 +386,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         for (int h = 0; h < 4; ++h) {
           uint32_t(&v)[16] = s[h & 1];
           tmem_ld_wait();
+          if (16 * h >= most) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[8 * h + i] = 0u;
+            continue;
+          }
           if (h < 3) tmem_ld_32x16(s_tmem + 64u * half + 16u * (h + 1), s[(h + 1) & 1]);
           if (masked) {
 #pragma unroll
@@ -380,17 +458,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (mine) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
-          if (odd)   // rare: a key of an edge tile has elements that are not finite
-            for (int key = 128 * edge0; key < lim; ++key)
-              if ((odd_keys[(key - 128 * edge0) >> 5] >> (key & 31)) & 1u) {
-                const uint16_t* v = static_cast<const uint16_t*>(a.v) + int64_t(k0 + key) * a.kv_stride + int64_t(g) * a.D + (D / 2) * half + 32 * h;
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if ((D / 2) * half + 32 * h + i < a.D && (odd_halves<BF16>(v[i]) & 0xffffu)) {
-                    const float f = BF16 ? __uint_as_float(uint32_t(v[i]) << 16) : __half2float(__ushort_as_half(v[i]));
-                    o[i] = __float_as_uint(__uint_as_float(o[i]) + f);
-                  }
-              }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint4 w;
@@ -410,13 +477,28 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         __syncwarp();
       }
+      if (odd && mine) {   // rare: what the edge tiles' V has that is not finite, to the rows that see it
+        uint16_t* o16 = reinterpret_cast<uint16_t*>(out);
+        const int cols = min(D / 2, a.D - (D / 2) * half);
+#pragma unroll 1
+        for (int key = 128 * edge0; key < lim; ++key) {
+          if (!((odd_keys[(key - 128 * edge0) >> 5] >> (key & 31)) & 1u)) continue;
+          const uint16_t* v = static_cast<const uint16_t*>(a.v) + int64_t(k0 + key) * a.kv_stride + int64_t(g) * a.D + (D / 2) * half;
+#pragma unroll 1
+          for (int i = 0; i < cols; ++i)
+            if (odd_halves<BF16>(v[i]) & 0xffffu) {
+              const float sum = to_16<BF16>(o16[i]) + to_16<BF16>(v[i]);
+              o16[i] = uint16_t(pack2<BF16>(sum, 0.0f));
+            }
+        }
+      }
     }
   }
   tc_fence_before_sync();
   __syncthreads();
   if (warp == W_MMA) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, Sh::TMEM);
   }
 }
 
@@ -439,6 +521,17 @@ int attn_tensor_map(CUtensorMap* map, bool bf16, const void* p, int64_t rows, in
   return SIMP_OK;
 }
 
+template <bool BF16, int D, int TILES>
+static int tc_run(const TcArgs& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv) {
+  using Sh = TcShape<D, TILES>;
+  const AttnPromptArgs& a = p.a;
+  auto kern = attn_prompt_tc_kernel<BF16, D, TILES>;
+  SIMP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Sh::SMEM)));
+  const int64_t units = std::min(a.total_q, a.total_q / (TILES * p.tpt) + a.n_seqs) * a.G;
+  SIMP_REQUIRE(units <= INT_MAX, SIMP_ERR_SHAPE, "attn_prompt: too many rows and heads");
+  SIMP_CUDA(launch_kernel(kern, dim3(unsigned(units)), dim3(Sh::THREADS), Sh::SMEM, ctx().stream, true, mq, mk, mv, p));
+  return SIMP_OK;
+}
 template <bool BF16, int D>
 static int tc_launch(TcArgs p) {
   const AttnPromptArgs& a = p.a;
@@ -447,13 +540,10 @@ static int tc_launch(TcArgs p) {
   if (int rc = attn_tensor_map(&mq, BF16, p.q, a.total_q, a.H, D, p.q_stride, a.rep, p.tpt)) return rc;
   if (int rc = attn_tensor_map(&mk, BF16, p.k, a.total_k, a.G, D, p.kv_stride, 1, 128)) return rc;
   if (int rc = attn_tensor_map(&mv, BF16, p.v, a.total_k, a.G, D, p.kv_stride, 1, 128)) return rc;
-  auto kern = attn_prompt_tc_kernel<BF16, D>;
-  SIMP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(TcShape<D>::SMEM)));
-  const int64_t units = std::min(a.total_q, a.total_q / (2 * p.tpt) + a.n_seqs) * a.G;
-  SIMP_REQUIRE(units <= INT_MAX, SIMP_ERR_SHAPE, "attn_prompt: too many rows and heads");
-  kern<<<unsigned(units), TC_THREADS, TcShape<D>::SMEM, ctx().stream>>>(mq, mk, mv, p);
-  SIMP_LAUNCH_CHECK();
-  return SIMP_OK;
+  // Short prompts on one tile per block and two blocks per SM.  32/8 heads, us with one / two tiles: D = 64, 64 prompts of 128
+  // tokens 64 / 73, 16 of 512 86 / 88, 4 of 2048 172 / 172; D = 128, 64 of 1 17 / 28, 64 of 128 88 / 97, 32 of 256 101 / 96.
+  const bool brief = a.total_k < (D == 64 ? 2048 : 192) * int64_t(a.n_seqs);
+  return brief ? tc_run<BF16, D, 1>(p, mq, mk, mv) : tc_run<BF16, D, 2>(p, mq, mk, mv);
 }
 
 // Rows to rows of heads padded to DP elements.  16-bit types are copied; f32 is split into three bf16 planes h + m + l (8 bits
@@ -464,6 +554,8 @@ template <bool SPLIT>
 __global__ void __launch_bounds__(256) attn_pack_kernel(const void* __restrict__ src, uint16_t* __restrict__ dst, int64_t rows, int heads, int D,
                                                         int DP, int64_t stride, uint8_t* __restrict__ odd, int* any) {
   const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;   // eighth of a padded row
+  pdl_launch_dependents();
+  pdl_wait();
   const int eighths = DP / 8, per = heads * eighths;
   const int64_t row = i / per;
   const bool in = row < rows;
@@ -509,8 +601,7 @@ int attn_pack(bool split, const void* src, void* dst, int64_t rows, int heads, i
   SIMP_REQUIRE(n <= INT_MAX, SIMP_ERR_SHAPE, "attn_prompt: too many rows and heads");
   if (n == 0) return SIMP_OK;
   auto kern = split ? attn_pack_kernel<true> : attn_pack_kernel<false>;
-  kern<<<unsigned(n), 256, 0, ctx().stream>>>(src, static_cast<uint16_t*>(dst), rows, heads, D, DP, stride, odd, any);
-  SIMP_LAUNCH_CHECK();
+  SIMP_CUDA(launch_kernel(kern, dim3(unsigned(n)), dim3(256), 0, ctx().stream, true, src, static_cast<uint16_t*>(dst), rows, heads, D, DP, stride, odd, any));
   return SIMP_OK;
 }
 

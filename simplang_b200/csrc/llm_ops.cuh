@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace simp {
@@ -71,12 +73,34 @@ __device__ __forceinline__ bool seq_range(const int32_t* off, int s, int64_t tot
 
 // Finds the sequence and the place in it of work unit u when sequence s has count(s) units (called by a whole warp;
 // every lane gets the result).  32 sequences are looked at together, so a batch of 64 costs two rounds.  False: u lies
-// behind the last unit.
-template <typename Count>
-__device__ __forceinline__ bool find_unit(int64_t u, int n_seqs, Count count, int& seq, int& place) {
+// behind the last unit.  With `weight`, up to 32 sequences are taken in the order of falling weight: blocks start in the
+// order of their numbers, and long work that starts last ends alone.
+struct NoWeight {};
+template <typename Count, typename Weight = NoWeight>
+__device__ __forceinline__ bool find_unit(int64_t u, int n_seqs, Count count, int& seq, int& place, Weight weight = Weight()) {
   const int lane = threadIdx.x & 31;
   for (int s0 = 0; s0 < n_seqs; s0 += 32) {
-    const int c = s0 + lane < n_seqs ? count(s0 + lane) : 0;
+    int c = s0 + lane < n_seqs ? count(s0 + lane) : 0, which = lane;
+    if constexpr (!std::is_same_v<Weight, NoWeight>) {
+      if (n_seqs > 1 && n_seqs <= 32) {
+        // weight and lane in one word, sorted by comparators at distances k / 2, k / 4 .. 1 of runs of k = 2, 4 .. 32 (Batcher's
+        // bitonic network): falling weight, equal ones by their numbers, lanes behind the last sequence at the end
+        uint32_t key = (lane < n_seqs ? uint32_t(min(max(weight(lane), 0) + 1, (1 << 27) - 1)) << 5 : 0u) | uint32_t(31 - lane);
+        const uint32_t head = __shfl_sync(0xffffffffu, key, 0) >> 5;
+        if (!__all_sync(0xffffffffu, lane >= n_seqs || key >> 5 == head)) {
+#pragma unroll
+          for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+            for (int d = k >> 1; d > 0; d >>= 1) {
+              const uint32_t o = __shfl_xor_sync(0xffffffffu, key, d);
+              const bool larger = ((lane & d) == 0) == ((lane & k) == 0);
+              key = larger ? max(key, o) : min(key, o);
+            }
+          which = 31 - int(key & 31u);
+          c = __shfl_sync(0xffffffffu, c, which);
+        }
+      }
+    }
     int64_t upto = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -86,7 +110,7 @@ __device__ __forceinline__ bool find_unit(int64_t u, int n_seqs, Count count, in
     const unsigned in = __ballot_sync(0xffffffffu, u < upto);
     if (in) {
       const int l = __ffs(in) - 1;
-      seq = s0 + l;
+      seq = s0 + __shfl_sync(0xffffffffu, which, l);
       place = int(u - __shfl_sync(0xffffffffu, upto - c, l));
       return true;
     }
