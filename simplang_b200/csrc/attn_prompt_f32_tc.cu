@@ -3,15 +3,16 @@
 // q, k and v are split into three bf16 planes each (x = h + m + l, 24 bits), and a product is the six plane products of
 // relative size 2^-16 and above: l.h, h.l, m.m, m.h, h.m, h.h.  The tensor cores add into their f32 accumulators with
 // truncation, so (1) the small products come first and only the last eighth or less of the additions is made at full
-// size, and (2) the output of every tile of 64 keys is a sum of its own, added to f32 registers with rounding: an
+// size, and (2) the output of every tile of keys is a sum of its own, added to f32 registers with rounding: an
 // accumulator kept over a long prompt would drift by 2e-8 per instruction.
 //
 // One block of 12 warps per row tile (128 rows: 128 / rep tokens x the rep heads that share a key/value head):
-//   warp 0      TMA: the planes of Q once, of K and V per tile of 64 keys
-//   warp 1      MMAs: S = Q K^T (128 x 64) as soon as the softmax has read the S before; T = P V into a TMEM tile
-//   warps 4-11  softmax, two threads per row (32 keys each); P in three planes to TMEM; T into registers (D / 2 each)
-// Per tile the tensor cores need 6 x (D / 16 x 48 + 4 x D / 2) cycles (the first is bound by shared memory: 6 KB per 48
-// cycles), for D = 128 3840, the softmax about 2500 beside them.
+//   warp 0      TMA: the planes of K and V per tile of 64 keys (head sizes up to 64: 128), two stages of 48 KB each
+//   warp 1      MMAs: S = Q K^T as soon as the softmax has read the S before; T = P V into a TMEM tile
+//   warps 4-11  softmax, two threads per row; P in three planes to TMEM; T into registers (D / 2 each)
+// The planes of Q lie in TMEM: from shared memory they would be read again for every product (6 KB per MMA of 32 cycles,
+// where shared memory gives 128 bytes a cycle: 77 cycles were measured), and there would be no room for second stages.
+// Per tile the tensor cores need 3072 cycles, the softmax about as many beside them.
 //
 // No plane product of an infinity or a NaN is right, and a zero weight does not hide them from an MMA (a tile may hold keys
 // that some rows must not see, or rows of the next sequence).  The splitting pass leaves them out of the planes and marks
@@ -24,20 +25,22 @@
 
 namespace simp {
 
-constexpr int F3_THREADS = 384, F3_KEYS = 64;
+constexpr int F3_THREADS = 384;
 
 template <int D>
 struct F3Shape {
-  static constexpr int QPLANE = 128 * D * 2, KPLANE = F3_KEYS * D * 2;
-  static constexpr int BARS = 9;
-  static constexpr size_t SMEM = 3 * size_t(QPLANE) + 6 * size_t(KPLANE) + BARS * 8 + 16 + 8 * 128 + 24;
-  static constexpr uint32_t TMEM = D == 64 ? 256 : 512, P = 64, T = D == 64 ? 160 : 256;   // columns: S at 0, three P planes, T
+  static constexpr int KEYS = D == 64 ? 128 : 64, ATOM = KEYS * 128;   // bytes of 64 elements of a tile's rows
+  static constexpr int PLANE = KEYS * D * 2, STAGE = 3 * PLANE;
+  static constexpr int BARS = 13;
+  static constexpr size_t SMEM = 4 * size_t(STAGE) + BARS * 8 + 16 + 8 * 128 + 24;
+  static constexpr uint32_t P = KEYS, T = P + 3 * KEYS / 2, Q = T + D;   // TMEM columns: S, three planes of P, T, three planes of Q
+  static_assert(Q + 3 * D / 2 <= 512 && SMEM <= 232448, "");
 };
-static_assert(F3Shape<128>::SMEM <= 232448 && 2 * F3Shape<64>::SMEM <= 228 * 1024 - 2048, "");
 
 struct F3Args {
   AttnPromptArgs a;
   int tpt;
+  const uint16_t* q;   // planes [3][total_q][H][D]
   const int* any;   // set: some element is not finite; then the bytes of its row and head are set:
   const uint8_t *odd_q, *odd_k, *odd_v;
 };
@@ -50,15 +53,18 @@ __device__ __forceinline__ uint32_t tmem_ld_1(uint32_t t) {
 __device__ __forceinline__ void tmem_st_1(uint32_t t, uint32_t v) { asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(t), "r"(v) : "memory"); }
 
 template <int D>
-__global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
-    attn_prompt_f32_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                              const __grid_constant__ CUtensorMap map_v, const F3Args p) {
+__global__ void __launch_bounds__(F3_THREADS, 1)
+    attn_prompt_f32_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const F3Args p) {
   using Sh = F3Shape<D>;
+  constexpr int KEYS = Sh::KEYS, MINE = KEYS / 2;   // keys of a tile, of a thread
   extern __shared__ __align__(1024) uint8_t f3_raw[];
-  const uint32_t base = smem_u32(f3_raw), q_smem = base, k_smem = base + 3 * Sh::QPLANE, v_smem = k_smem + 3 * Sh::KPLANE, bars = v_smem + 3 * Sh::KPLANE;
-  const uint32_t q_bar = bars, k_full = bars + 8, k_empty = bars + 16, v_full = bars + 24, v_empty = bars + 32, s_bar = bars + 40, s_read = bars + 48,
-                 p_bar = bars + 56, t_bar = bars + 64;
-  uint8_t* tail = f3_raw + (bars - base) + Sh::BARS * 8;
+  const uint32_t base = smem_u32(f3_raw), k_smem = base, v_smem = base + 2 * Sh::STAGE, bars = base + 4 * Sh::STAGE;
+  auto k_full = [&](int s) { return bars + 8u * s; };
+  auto k_empty = [&](int s) { return bars + 16u + 8u * s; };
+  auto v_full = [&](int s) { return bars + 32u + 8u * s; };
+  auto v_empty = [&](int s) { return bars + 48u + 8u * s; };
+  const uint32_t s_bar = bars + 64, s_read = bars + 72, p_bar = bars + 80, t_bar = bars + 88, q_bar = bars + 96;
+  uint8_t* tail = f3_raw + 4 * Sh::STAGE + Sh::BARS * 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8);
   float* half_row = reinterpret_cast<float*>(tail + 16);   // [half][row]
@@ -70,15 +76,17 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
     return;
   }
   if (threadIdx.x == 0) {
-    mbar_init(q_bar, 1);
-    mbar_init(k_full, 1);
-    mbar_init(k_empty, 1);
-    mbar_init(v_full, 1);
-    mbar_init(v_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full(i), 1);
+      mbar_init(k_empty(i), 1);
+      mbar_init(v_full(i), 1);
+      mbar_init(v_empty(i), 1);
+    }
     mbar_init(s_bar, 1);
     mbar_init(s_read, 8);
     mbar_init(p_bar, 8);
     mbar_init(t_bar, 1);
+    mbar_init(q_bar, 8);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -109,7 +117,7 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
     }
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), Sh::TMEM);
+    tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
   tc_fence_before_sync();
@@ -117,7 +125,7 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   if (!found_unit[0]) {
-    if (warp == 1) tmem_dealloc(tmem, Sh::TMEM);
+    if (warp == 1) tmem_dealloc(tmem, 512);
     return;
   }
   q0 = found_unit[2];
@@ -129,27 +137,23 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
   const int r0 = ((nq + p.tpt - 1) / p.tpt - 1 - place) * p.tpt;   // the longest rows first
   const int64_t shift = int64_t(nk) - nq;
   auto sees = [&](int token) { return int(max(int64_t(0), min(int64_t(nk), token + shift + 1))); };
-  const int n = (sees(min(r0 + p.tpt, nq) - 1) + F3_KEYS - 1) / F3_KEYS;
+  const int n = (sees(min(r0 + p.tpt, nq) - 1) + KEYS - 1) / KEYS;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ loads
     if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(q_bar, 3 * (D / 64) * uint32_t(p.tpt * a.rep) * 128u);
-      for (int s = 0; s < 3; ++s)
-        for (int b = 0; b < D / 64; ++b)
-          tma_load_3d(q_smem + s * Sh::QPLANE + b * 16384, &map_q, q_bar, 64 * b, g * a.rep, int(s * a.total_q) + q0 + r0);
       bool ok = true;
       auto tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, uint32_t empty, int j) {
-        ok = ok && wait_bar(empty, (j & 1) ^ 1, abort_flag, a.status, 71);
+        ok = ok && wait_bar(empty, ((j >> 1) & 1) ^ 1, abort_flag, a.status, 71);
         if (!ok) return;
-        mbar_arrive_expect_tx(full, 3 * Sh::KPLANE);
+        mbar_arrive_expect_tx(full, Sh::STAGE);
         for (int s = 0; s < 3; ++s)
           for (int b = 0; b < D / 64; ++b)
-            tma_load_3d(dst + s * Sh::KPLANE + b * 8192, map, full, 64 * b, g, int(s * a.total_k) + k0 + F3_KEYS * j);
+            tma_load_3d(dst + (j & 1) * Sh::STAGE + s * Sh::PLANE + b * Sh::ATOM, map, full, 64 * b, g, int(s * a.total_k) + k0 + KEYS * j);
       };
       for (int j = 0; ok && j < n; ++j) {
-        tile(&map_k, k_smem, k_full, k_empty, j);
-        tile(&map_v, v_smem, v_full, v_empty, j);
+        tile(&map_k, k_smem, k_full(j & 1), k_empty(j & 1), j);
+        tile(&map_v, v_smem, v_full(j & 1), v_empty(j & 1), j);
       }
       if (!ok)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);   // let copies in flight land before the block retires
@@ -157,7 +161,9 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMAs (the whole warp with the same values, one lane issues)
-    constexpr uint32_t idesc_s = idesc_f16(true, F3_KEYS, false), idesc_t = idesc_f16(true, D, true);
+    constexpr uint32_t idesc_s = idesc_f16(true, KEYS, false);
+    const int width = (a.D + 15) / 16;                        // steps of 16 elements that hold something
+    const uint32_t idesc_t = idesc_f16(true, 16 * width, true);
     const bool leader = lane == 0;
     auto wait = [&](uint32_t bar, uint32_t phase, int site) {
       const bool ok = __all_sync(0xffffffffu, wait_bar(bar, phase, abort_flag, a.status, site));
@@ -166,50 +172,52 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
     };
     // planes of the two operands, small products first
     constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
-    auto scores = [&] {
-      const uint64_t qd = make_smem_desc_sw128(q_smem, 16u, 1024u), kd = make_smem_desc_sw128(k_smem, 16u, 1024u);
+    auto scores = [&](int j) {
+      const uint64_t kd = make_smem_desc_sw128(k_smem, 16u, 1024u) + uint64_t((j & 1) * (Sh::STAGE / 16));
 #pragma unroll
       for (int t = 0; t < 6; ++t)
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-          mma_f16_ss(tmem, qd + uint64_t(PA[t] * (Sh::QPLANE / 16) + (s >> 2) * 1024 + (s & 3) * 2),
-                     kd + uint64_t(PB[t] * (Sh::KPLANE / 16) + (s >> 2) * 512 + (s & 3) * 2), idesc_s, t > 0 || s > 0, leader);
+          if (s < width)
+            mma_f16_ts(tmem, tmem + Sh::Q + uint32_t(D / 2) * PA[t] + 8u * s, kd + uint64_t(PB[t] * (Sh::PLANE / 16) + (s >> 2) * (Sh::ATOM / 16) + (s & 3) * 2),
+                       idesc_s, t > 0 || s > 0, leader);
     };
-    auto values = [&] {
-      const uint64_t vd = make_smem_desc_sw128(v_smem, 8192u, 1024u);   // 64-element atoms 8 KB apart, 8 keys 1 KB apart
+    auto values = [&](int j) {
+      const uint64_t vd = make_smem_desc_sw128(v_smem, uint32_t(Sh::ATOM), 1024u) + uint64_t((j & 1) * (Sh::STAGE / 16));   // 8 keys 1 KB apart
 #pragma unroll
       for (int t = 0; t < 6; ++t)
 #pragma unroll
-        for (int s = 0; s < F3_KEYS / 16; ++s)
-          mma_f16_ts(tmem + Sh::T, tmem + Sh::P + 32u * PA[t] + 8u * s, vd + uint64_t(PB[t] * (Sh::KPLANE / 16) + s * 128), idesc_t, t > 0 || s > 0, leader);
+        for (int s = 0; s < KEYS / 16; ++s)
+          mma_f16_ts(tmem + Sh::T, tmem + Sh::P + uint32_t(KEYS / 2) * PA[t] + 8u * s, vd + uint64_t(PB[t] * (Sh::PLANE / 16) + s * 128), idesc_t, t > 0 || s > 0,
+                     leader);
     };
     bool ok = true;
     if (n > 0) {
-      ok = wait(q_bar, 0, 72) && wait(k_full, 0, 73);
+      ok = wait(q_bar, 0, 72) && wait(k_full(0), 0, 73);
       if (ok) {
-        scores();
+        scores(0);
         if (leader) {
           mma_commit(s_bar);
-          mma_commit(k_empty);
+          mma_commit(k_empty(0));
         }
       }
     }
     for (int j = 0; ok && j < n; ++j) {
       if (j + 1 < n) {
-        ok = wait(k_full, (j + 1) & 1, 74) && wait(s_read, j & 1, 75);
+        ok = wait(k_full((j + 1) & 1), ((j + 1) >> 1) & 1, 74) && wait(s_read, j & 1, 75);
         if (!ok) break;
-        scores();
+        scores(j + 1);
         if (leader) {
           mma_commit(s_bar);
-          mma_commit(k_empty);
+          mma_commit(k_empty((j + 1) & 1));
         }
       }
-      ok = wait(v_full, j & 1, 76) && wait(p_bar, j & 1, 77);
+      ok = wait(v_full(j & 1), (j >> 1) & 1, 76) && wait(p_bar, j & 1, 77);
       if (!ok) break;
-      values();
+      values(j);
       if (leader) {
         mma_commit(t_bar);
-        mma_commit(v_empty);
+        mma_commit(v_empty(j & 1));
       }
     }
     if (!ok)
@@ -219,12 +227,28 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
     // ------------------------------------------------------------------ softmax and sums
     const int half = (warp - 4) >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-    const uint32_t s_tmem = tmem + lanes + 32u * half, t_tmem = tmem + Sh::T + lanes + uint32_t(D / 2) * half;
+    const uint32_t s_tmem = tmem + lanes + uint32_t(MINE) * half, t_tmem = tmem + Sh::T + lanes + uint32_t(D / 2) * half;
     const int token = r0 + row / a.rep, head = g * a.rep + row % a.rep;
     const bool mine = row < p.tpt * a.rep && token < nq;
     const int lim = mine ? sees(token) : 0;
     volatile float* to = half_row + half * 128 + row;
     volatile float* from = half_row + (half ^ 1) * 128 + row;
+    // this row's planes of Q, half a row per thread, to TMEM (rows behind the sequence: zeros)
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t(q) * a.total_q + q0 + token) * a.H * D + int64_t(head) * D + (D / 2) * half);
+#pragma unroll
+      for (int h = 0; h < D / 32; ++h) {   // 16 elements
+        uint32_t w[8];
+        const uint4 x = mine ? __ldg(src + 2 * h) : make_uint4(0u, 0u, 0u, 0u), y = mine ? __ldg(src + 2 * h + 1) : make_uint4(0u, 0u, 0u, 0u);
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+        tmem_st_32x8(tmem + lanes + Sh::Q + uint32_t(D / 2) * q + uint32_t(D / 4) * half + 8u * h, w);
+      }
+    }
+    tmem_st_wait();
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_bar);
     const bool any = __ldcg(p.any) != 0, odd_row = any && mine && p.odd_q[int64_t(q0 + token) * a.H + head];
     float m = -INFINITY, l = 0.0f, o[D / 2];
 #pragma unroll
@@ -245,8 +269,8 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
       tc_fence_after_sync();
       if (any) {   // rare: scores of rows that are not finite, by the f32 tensors
 #pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-          const int key = F3_KEYS * j + 32 * half + i;
+        for (int i = 0; i < MINE; ++i) {
+          const int key = KEYS * j + MINE * half + i;
           uint32_t v = tmem_ld_1(s_tmem + i);
           tmem_ld_wait();
           if (key < lim && (odd_row || p.odd_k[int64_t(k0 + key) * a.G + g])) {
@@ -262,13 +286,14 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
         }
         tmem_st_wait();
       }
-      uint32_t s[32];
-      tmem_ld_32x32(s_tmem, s);
+      uint32_t s[MINE];
+#pragma unroll
+      for (int h = 0; h < MINE / 32; ++h) tmem_ld_32x32(s_tmem + 32u * h, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * h));
       tmem_ld_wait();
-      const int see = lim - F3_KEYS * j - 32 * half;
+      const int see = lim - KEYS * j - MINE * half;
       float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
+      for (int i = 0; i < MINE; ++i) {
         const float y = i < see ? __uint_as_float(s[i]) * a.scale_log2 : -INFINITY;
         s[i] = __float_as_uint(y);
         top = fmaxf(top, y);
@@ -281,43 +306,27 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
       const float mn = fmaxf(m, fmaxf(top, *from)), off = mn == -INFINITY ? 0.0f : mn;
       const float alpha = ex2(m - off);   // 0 for the first tile
       m = mn;
-      // The tile before: when it is done, its sum is taken and its P may be overwritten.  With D = 64 two blocks share the
-      // SM and 80 registers hold either the planes or what follows, so this comes first; with D = 128 the exponentials do,
-      // beside the MMAs of the tile before.
-      auto take = [&] {
-        if (j == 0) return;
+      float sum = 0.0f;
+      uint32_t w[3][MINE / 2];
+#pragma unroll
+      for (int i = 0; i < MINE / 2; ++i) {
+        const float e0 = ex2(__uint_as_float(s[2 * i]) - off), e1 = ex2(__uint_as_float(s[2 * i + 1]) - off);
+        sum += e0 + e1;
+        w[0][i] = pack2<true>(e0, e1);
+        const float f0 = e0 - __uint_as_float(w[0][i] << 16), f1 = e1 - __uint_as_float(w[0][i] & 0xffff0000u);
+        w[1][i] = pack2<true>(f0, f1);
+        w[2][i] = pack2<true>(f0 - __uint_as_float(w[1][i] << 16), f1 - __uint_as_float(w[1][i] & 0xffff0000u));
+      }
+      if (j > 0) {   // the tile before: when it is done, its sum is taken and its P may be overwritten
         ok = __all_sync(0xffffffffu, wait_bar(t_bar, (j - 1) & 1, abort_flag, a.status, 79)) && ok;
         tc_fence_after_sync();
         add_tile(alpha);
-      };
-      float sum = 0.0f;
-      auto planes = [&](int i, uint32_t& w0, uint32_t& w1, uint32_t& w2) {   // two weights: three planes
-        const float e0 = ex2(__uint_as_float(s[2 * i]) - off), e1 = ex2(__uint_as_float(s[2 * i + 1]) - off);
-        sum += e0 + e1;
-        w0 = pack2<true>(e0, e1);
-        const float f0 = e0 - __uint_as_float(w0 << 16), f1 = e1 - __uint_as_float(w0 & 0xffff0000u);
-        w1 = pack2<true>(f0, f1);
-        w2 = pack2<true>(f0 - __uint_as_float(w1 << 16), f1 - __uint_as_float(w1 & 0xffff0000u));
-      };
-      const uint32_t p_tmem = tmem + lanes + Sh::P + 16u * half;
-      if (D == 64) {
-        take();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t w[3][8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) planes(8 * h + i, w[0][i], w[1][i], w[2][i]);
-#pragma unroll
-          for (int q = 0; q < 3; ++q) tmem_st_32x8(p_tmem + 32u * q + 8u * h, w[q]);
-        }
-      } else {
-        uint32_t w[3][16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) planes(i, w[0][i], w[1][i], w[2][i]);
-        take();
-#pragma unroll
-        for (int q = 0; q < 3; ++q) tmem_st_32x16(p_tmem + 32u * q, w[q]);
       }
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int h = 0; h < MINE / 32; ++h)
+          tmem_st_32x16(tmem + lanes + Sh::P + uint32_t(KEYS / 2) * q + uint32_t(MINE / 2) * half + 16u * h, *reinterpret_cast<uint32_t(*)[16]>(w[q] + 16 * h));
       l = fmaf(l, alpha, sum);
       tmem_st_wait();
       tc_fence_before_sync();
@@ -364,7 +373,7 @@ __global__ void __launch_bounds__(F3_THREADS, D == 64 ? 2 : 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, Sh::TMEM);
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -372,15 +381,15 @@ template <int D>
 static int f3_launch(F3Args p, const uint8_t* q, const uint8_t* k, const uint8_t* v) {
   const AttnPromptArgs& a = p.a;
   p.tpt = 128 / a.rep;
-  CUtensorMap mq, mk, mv;
-  if (int rc = attn_tensor_map(&mq, true, q, 3 * a.total_q, a.H, D, int64_t(a.H) * D, a.rep, p.tpt)) return rc;
-  if (int rc = attn_tensor_map(&mk, true, k, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, F3_KEYS)) return rc;
-  if (int rc = attn_tensor_map(&mv, true, v, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, F3_KEYS)) return rc;
+  p.q = reinterpret_cast<const uint16_t*>(q);
+  CUtensorMap mk, mv;
+  if (int rc = attn_tensor_map(&mk, true, k, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, F3Shape<D>::KEYS)) return rc;
+  if (int rc = attn_tensor_map(&mv, true, v, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, F3Shape<D>::KEYS)) return rc;
   auto kern = attn_prompt_f32_tc_kernel<D>;
   SIMP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(F3Shape<D>::SMEM)));
   const int64_t units = std::min(a.total_q, a.total_q / p.tpt + a.n_seqs) * a.G;
   SIMP_REQUIRE(units <= INT_MAX, SIMP_ERR_SHAPE, "attn_prompt: too many rows and heads");
-  SIMP_CUDA(launch_kernel(kern, dim3(unsigned(units)), dim3(F3_THREADS), F3Shape<D>::SMEM, ctx().stream, true, mq, mk, mv, p));
+  SIMP_CUDA(launch_kernel(kern, dim3(unsigned(units)), dim3(F3_THREADS), F3Shape<D>::SMEM, ctx().stream, true, mk, mv, p));
   return SIMP_OK;
 }
 
