@@ -21,6 +21,13 @@ struct AttnPromptArgs {
 int attn_prompt_tc(const AttnPromptArgs& a, int dtype);    // 16-bit types
 int attn_prompt_f32_tc(const AttnPromptArgs& a);           // f32
 // Rows to padded rows (f32: three bf16 planes), see attn_prompt_tc.cu.
-int attn_pack(bool split, const void* src, void* dst, int64_t rows, int heads, int D, int DP, int64_t stride, uint8_t* odd, int* any);
+struct AttnPack {
+  const void* src;
+  void* dst;
+  uint8_t* odd;   // f32: per row and head, whether something is not finite
+  int64_t rows, stride;
+  int heads;
+};
+int attn_pack(bool split, const AttnPack& q, const AttnPack& k, const AttnPack& v, int D, int DP, int* any);
 
 }  // namespace simp

@@ -117,13 +117,13 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
     }
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_alloc(smem_u32(tmem_slot), 512);   // (all: one block per SM)
     tmem_relinquish();
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;   // the block allocates every column
   if (!found_unit[0]) {
     if (warp == 1) tmem_dealloc(tmem, 512);
     return;
@@ -178,9 +178,8 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
       for (int t = 0; t < 6; ++t)
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-          if (s < width)
-            mma_f16_ts(tmem, tmem + Sh::Q + uint32_t(D / 2) * PA[t] + 8u * s, kd + uint64_t(PB[t] * (Sh::PLANE / 16) + (s >> 2) * (Sh::ATOM / 16) + (s & 3) * 2),
-                       idesc_s, t > 0 || s > 0, leader);
+          mma_f16_ts(tmem, tmem + Sh::Q + uint32_t(D / 2) * PA[t] + 8u * s, kd + uint64_t(PB[t] * (Sh::PLANE / 16) + (s >> 2) * (Sh::ATOM / 16) + (s & 3) * 2),
+                     idesc_s, t > 0 || s > 0, leader && s < width);
     };
     auto values = [&](int j) {
       const uint64_t vd = make_smem_desc_sw128(v_smem, uint32_t(Sh::ATOM), 1024u) + uint64_t((j & 1) * (Sh::STAGE / 16));   // 8 keys 1 KB apart
@@ -409,9 +408,8 @@ int attn_prompt_f32_tc(const AttnPromptArgs& a) {
   p.odd_v = ov;
   int* flag = reinterpret_cast<int*>(any);
   SIMP_CUDA(cudaMemsetAsync(flag, 0, 4, ctx().stream));
-  if (int rc = attn_pack(true, a.q, q, a.total_q, a.H, a.D, D, a.q_stride, oq, flag)) return rc;
-  if (int rc = attn_pack(true, a.k, k, a.total_k, a.G, a.D, D, a.kv_stride, ok, flag)) return rc;
-  if (int rc = attn_pack(true, a.v, v, a.total_k, a.G, a.D, D, a.kv_stride, ov, flag)) return rc;
+  const AttnPack of_q{a.q, q, oq, a.total_q, a.q_stride, a.H}, of_k{a.k, k, ok, a.total_k, a.kv_stride, a.G}, of_v{a.v, v, ov, a.total_k, a.kv_stride, a.G};
+  if (int rc = attn_pack(true, of_q, of_k, of_v, a.D, D, flag)) return rc;
   return D == 64 ? f3_launch<64>(p, q, k, v) : f3_launch<128>(p, q, k, v);
 }
 

@@ -22,6 +22,7 @@
 // per such key tells the epilogue to add those elements (read again from global memory) to the rows that do see the key.
 #include <algorithm>
 #include <climits>
+#include <cstring>
 #include <type_traits>
 
 #include "attn_tc.cuh"
@@ -63,7 +64,7 @@ struct TcArgs {
   const void* k;
   const void* v;
   int64_t q_stride, kv_stride;
-  bool whole;       // outputs are written 16 bytes at a time: a.D == D, aligned rows
+  int chunk;        // elements of an output row that are written together: 8, 4 or 1, by its alignment and head size
 };
 
 // bits of the 16-bit halves of w that are infinity or NaN
@@ -465,13 +466,18 @@ __global__ void __launch_bounds__(128 + 256 * TILES, 3 - TILES)
             w.y = pack2<BF16>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
             w.z = pack2<BF16>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
             w.w = pack2<BF16>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
-            if (p.whole) {
-              *reinterpret_cast<uint4*>(out + 64 * h + 16 * i) = w;
+            const int left = a.D - ((D / 2) * half + 32 * h + 8 * i);   // elements from here to the head's end
+            uint8_t* at = out + 64 * h + 16 * i;
+            if (p.chunk == 8) {
+              if (left > 0) *reinterpret_cast<uint4*>(at) = w;
+            } else if (p.chunk == 4) {
+              if (left > 0) *reinterpret_cast<uint2*>(at) = make_uint2(w.x, w.y);
+              if (left > 4) *reinterpret_cast<uint2*>(at + 8) = make_uint2(w.z, w.w);
             } else {
               const uint16_t* e = reinterpret_cast<const uint16_t*>(&w);
 #pragma unroll
               for (int t = 0; t < 8; ++t)
-                if ((D / 2) * half + 32 * h + 8 * i + t < a.D) reinterpret_cast<uint16_t*>(out + 64 * h + 16 * i)[t] = e[t];
+                if (t < left) reinterpret_cast<uint16_t*>(at)[t] = e[t];
             }
           }
         }
@@ -549,26 +555,47 @@ static int tc_launch(TcArgs p) {
 // Rows to rows of heads padded to DP elements.  16-bit types are copied; f32 is split into three bf16 planes h + m + l (8 bits
 // of mantissa each: exact, but for what lies below 2^-133), one behind the other.  Elements that are not finite have no
 // place there: they are zeros in the planes, the byte of their row and head in `odd` is set, and *any.  A thread writes
-// eight elements, the DP / 8 threads of a head are neighbours in a warp.
-template <bool SPLIT>
-__global__ void __launch_bounds__(256) attn_pack_kernel(const void* __restrict__ src, uint16_t* __restrict__ dst, int64_t rows, int heads, int D,
-                                                        int DP, int64_t stride, uint8_t* __restrict__ odd, int* any) {
-  const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;   // eighth of a padded row
+// eight elements, the DP / 8 threads of a head are neighbours in a warp.  VEC: four elements lie together at a multiple of
+// their size (D and strides multiples of 4, aligned pointers).
+template <bool SPLIT, bool VEC>
+__global__ void __launch_bounds__(256) attn_pack_kernel(const AttnPack q, const AttnPack k, const AttnPack v, unsigned blocks_q, unsigned blocks_k, int D,
+                                                        int DP, int* any) {
   pdl_launch_dependents();
   pdl_wait();
+  unsigned block = blockIdx.x;
+  const AttnPack& t = block < blocks_q ? q : block < blocks_q + blocks_k ? k : v;
+  block -= block < blocks_q ? 0 : block < blocks_q + blocks_k ? blocks_q : blocks_q + blocks_k;
+  const void* __restrict__ src = t.src;
+  uint16_t* __restrict__ dst = static_cast<uint16_t*>(t.dst);
+  uint8_t* __restrict__ odd = t.odd;
+  const int64_t rows = t.rows, stride = t.stride;
+  const int heads = t.heads;
+  const int64_t i = int64_t(block) * blockDim.x + threadIdx.x;   // eighth of a padded row
   const int eighths = DP / 8, per = heads * eighths;
   const int64_t row = i / per;
   const bool in = row < rows;
   const int at = int(i - row * per), head = at / eighths, d0 = 8 * (at % eighths);
   const int64_t from = row * stride + int64_t(head) * D + d0;
   const int n = in ? min(8, D - d0) : 0;
+  using E = std::conditional_t<SPLIT, float, uint16_t>;
+  using V4 = std::conditional_t<SPLIT, float4, uint2>;
+  E e8[8];
+  if (VEC) {   // n is 8, 4 or 0 or less
+    V4 w[2] = {};
+    if (n > 0) w[0] = __ldcs(reinterpret_cast<const V4*>(static_cast<const E*>(src) + from));
+    if (n > 4) w[1] = __ldcs(reinterpret_cast<const V4*>(static_cast<const E*>(src) + from) + 1);
+    memcpy(e8, w, sizeof(e8));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) e8[e] = e < n ? static_cast<const E*>(src)[from + e] : E(0);
+  }
   uint4 out[3];
   uint16_t* h = reinterpret_cast<uint16_t*>(out);
   bool bad = false;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    if (SPLIT) {
-      float x = e < n ? static_cast<const float*>(src)[from + e] : 0.0f;
+    if constexpr (SPLIT) {
+      float x = e8[e];
       if (!(fabsf(x) <= 3.402823466e38f)) bad = true, x = 0.0f;
       uint16_t a = __bfloat16_as_ushort(__float2bfloat16_rn(x));
       if ((a & 0x7fffu) == 0x7f80u) --a;   // the largest f32 would round to infinity
@@ -578,7 +605,7 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(const void* __restrict__
       h[8 + e] = __bfloat16_as_ushort(b);
       h[16 + e] = __bfloat16_as_ushort(__float2bfloat16_rn(r - __bfloat162float(b)));
     } else {
-      h[e] = e < n ? static_cast<const uint16_t*>(src)[from + e] : uint16_t(0);
+      h[e] = e8[e];
     }
   }
   if (in) {
@@ -596,12 +623,14 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(const void* __restrict__
   }
 }
 
-int attn_pack(bool split, const void* src, void* dst, int64_t rows, int heads, int D, int DP, int64_t stride, uint8_t* odd, int* any) {
-  const int64_t n = cdiv(rows * heads * (DP / 8), 256);
-  SIMP_REQUIRE(n <= INT_MAX, SIMP_ERR_SHAPE, "attn_prompt: too many rows and heads");
-  if (n == 0) return SIMP_OK;
-  auto kern = split ? attn_pack_kernel<true> : attn_pack_kernel<false>;
-  SIMP_CUDA(launch_kernel(kern, dim3(unsigned(n)), dim3(256), 0, ctx().stream, true, src, static_cast<uint16_t*>(dst), rows, heads, D, DP, stride, odd, any));
+int attn_pack(bool split, const AttnPack& q, const AttnPack& k, const AttnPack& v, int D, int DP, int* any) {
+  auto blocks = [&](const AttnPack& t) { return cdiv(t.rows * t.heads * (DP / 8), 256); };
+  const int64_t nq = blocks(q), nk = blocks(k);
+  SIMP_REQUIRE(nq + 2 * nk <= INT_MAX, SIMP_ERR_SHAPE, "attn_prompt: too many rows and heads");
+  const size_t four = split ? 16 : 8;
+  const bool vec = D % 4 == 0 && q.stride % 4 == 0 && k.stride % 4 == 0 && aligned_to(q.src, four) && aligned_to(k.src, four) && aligned_to(v.src, four);
+  auto kern = split ? (vec ? attn_pack_kernel<true, true> : attn_pack_kernel<true, false>) : (vec ? attn_pack_kernel<false, true> : attn_pack_kernel<false, false>);
+  SIMP_CUDA(launch_kernel(kern, dim3(unsigned(nq + 2 * nk)), dim3(256), 0, ctx().stream, true, q, k, v, unsigned(nq), unsigned(nk), D, DP, any));
   return SIMP_OK;
 }
 
@@ -612,7 +641,7 @@ int attn_prompt_tc(const AttnPromptArgs& a, int dtype) {
   const int D = a.D <= 64 ? 64 : 128;
   TcArgs p{};
   p.a = a;
-  p.whole = a.D == D && aligned_to(a.out, 16) && a.out_stride % 8 == 0;
+  p.chunk = a.D % 8 == 0 && aligned_to(a.out, 16) && a.out_stride % 8 == 0 ? 8 : a.D % 4 == 0 && aligned_to(a.out, 8) && a.out_stride % 4 == 0 ? 4 : 1;
   p.q = a.q;
   p.k = a.k;
   p.v = a.v;
@@ -627,9 +656,9 @@ int attn_prompt_tc(const AttnPromptArgs& a, int dtype) {
     p.v = s + nq + nk;
     p.q_stride = int64_t(a.H) * D;
     p.kv_stride = int64_t(a.G) * D;
-    if (int rc = attn_pack(false, a.q, s, a.total_q, a.H, a.D, D, a.q_stride, nullptr, nullptr)) return rc;
-    if (int rc = attn_pack(false, a.k, s + nq, a.total_k, a.G, a.D, D, a.kv_stride, nullptr, nullptr)) return rc;
-    if (int rc = attn_pack(false, a.v, s + nq + nk, a.total_k, a.G, a.D, D, a.kv_stride, nullptr, nullptr)) return rc;
+    const AttnPack of_q{a.q, s, nullptr, a.total_q, a.q_stride, a.H}, of_k{a.k, s + nq, nullptr, a.total_k, a.kv_stride, a.G};
+    const AttnPack of_v{a.v, s + nq + nk, nullptr, a.total_k, a.kv_stride, a.G};
+    if (int rc = attn_pack(false, of_q, of_k, of_v, a.D, D, nullptr)) return rc;
   }
   if (dtype == SIMP_DTYPE_BF16) return D == 64 ? tc_launch<true, 64>(p) : tc_launch<true, 128>(p);
   return D == 64 ? tc_launch<false, 64>(p) : tc_launch<false, 128>(p);
