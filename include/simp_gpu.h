@@ -176,9 +176,12 @@ int simp_gpu_silu_f32(const float* x_dev, const float* mul_dev, float* y_dev, in
  * same sequence, nq and nk being its query and key rows: with nk > nq the queries are the last nq places of the text
  * (a prompt that goes on behind rows which kv8_read brought back).  k_offsets_dev NULL: the same as q_offsets_dev.  A
  * query row that sees no key (nk < nq) gets zeros.  Keys that a row does not see have no influence on it, NaN and
- * infinities included.  16-bit types with head_dim 64 or 128 whose rows TMA can address (16-byte pointers and strides)
- * run on the tcgen05 tensor cores, where the softmax weights are rounded to the 16-bit type before they multiply v;
- * everything else runs in f32 arithmetic.  The group n_heads / n_kv_heads is at most 128. */
+ * infinities included.  Runs on the tcgen05 tensor cores: 16-bit types as they are, the softmax weights rounded to the
+ * 16-bit type before they multiply v; f32 at f32 accuracy (each operand split into three bf16 numbers, six products).  The
+ * split operands (6 bytes per element, heads padded to 64 or 128), and padded copies of 16-bit rows that TMA cannot address
+ * (head_dim other than 64 and 128, pointers or strides off 16 bytes), lie in library scratch, grown on first use; inside a
+ * recording that would have to grow it, and for 16-bit types with scale <= 0, an FFMA kernel does the work instead.  The
+ * group n_heads / n_kv_heads is at most 128. */
 int simp_gpu_attn_prompt(const void* q_dev, const void* k_dev, const void* v_dev, void* out_dev, const int32_t* q_offsets_dev,
                          const int32_t* k_offsets_dev, int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t n_heads,
                          int64_t n_kv_heads, int64_t head_dim, int64_t q_stride, int64_t kv_stride, int64_t out_stride,
@@ -212,7 +215,7 @@ int simp_gpu_kv8_read(const simp_kv8_cache* cache, const int32_t* block_table_de
                       void* v_dev, int64_t kv_stride, const int32_t* offsets_dev, const int32_t* starts_dev, int64_t n_seqs,
                       int64_t total, int dtype);
 /* Attention of one query token per sequence, q and out [n_seqs, n_heads, head_dim], over the first lengths[s] (int32,
- * device, 0 .. max_len) places of its cache; max_len is at most table_stride * block_tokens.  A sequence of length 0
+ * device, 0 .. max_len) places of its cache; max_len is at most table_stride * block_tokens and 2^30.  A sequence of length 0
  * gets zeros.  Long caches are split over blocks of the GPU and joined in a fixed order (library scratch: make the first
  * call of a size before recording it). */
 int simp_gpu_attn_kv8(const simp_kv8_cache* cache, const int32_t* block_table_dev, int64_t table_stride, const void* q_dev,

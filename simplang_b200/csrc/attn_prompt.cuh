@@ -20,6 +20,12 @@ struct AttnPromptArgs {
 // Tensor-core forms; 1: the call is not for them (nothing was launched).
 int attn_prompt_tc(const AttnPromptArgs& a, int dtype);    // 16-bit types
 int attn_prompt_f32_tc(const AttnPromptArgs& a);           // f32
+// Scratch that is refused (inside a recording) or not to be had sends a call to the FFMA kernel, which needs none; the
+// allocation's error must not be taken for that launch's.
+inline int attn_no_scratch() {
+  cudaGetLastError();
+  return 1;
+}
 // Rows to padded rows (f32: three bf16 planes), see attn_prompt_tc.cu.
 struct AttnPack {
   const void* src;

@@ -398,7 +398,7 @@ int attn_prompt_f32_tc(const AttnPromptArgs& a) {
   const int D = a.D <= 64 ? 64 : 128;
   const size_t nq = size_t(a.total_q) * a.H, nk = size_t(a.total_k) * a.G, pad = 16;
   uint8_t* s = static_cast<uint8_t*>(scratch((nq + 2 * nk) * D * 6 + 4 * pad + nq + 2 * nk, SCRATCH_ATTN_PACK));
-  if (!s) return 1;
+  if (!s) return attn_no_scratch();
   uint8_t *q = s, *k = q + nq * D * 6, *v = k + nk * D * 6, *any = v + nk * D * 6, *oq = any + pad, *ok = oq + nq, *ov = ok + nk;
   F3Args p{};
   p.a = a;

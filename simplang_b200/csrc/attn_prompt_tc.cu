@@ -650,7 +650,7 @@ int attn_prompt_tc(const AttnPromptArgs& a, int dtype) {
   if (a.D != D || !aligned_to(a.q, 16) || !aligned_to(a.k, 16) || !aligned_to(a.v, 16) || a.q_stride % 8 || a.kv_stride % 8) {
     const size_t nq = size_t(a.total_q) * a.H * D * 2, nk = size_t(a.total_k) * a.G * D * 2;
     uint8_t* s = static_cast<uint8_t*>(scratch(nq + 2 * nk, SCRATCH_ATTN_PACK));
-    if (!s) return 1;
+    if (!s) return attn_no_scratch();
     p.q = s;
     p.k = s + nq;
     p.v = s + nq + nk;

@@ -857,6 +857,7 @@ SIMP_API int simp_gpu_attn_kv8(const simp_kv8_cache* cache, const int32_t* block
                (long long)n_heads, a.c.G);
   SIMP_REQUIRE(max_len <= table_stride * a.c.bt, SIMP_ERR_SHAPE, "attn_kv8: max_len %lld exceeds the table's %lld blocks of %d tokens",
                (long long)max_len, (long long)table_stride, a.c.bt);
+  SIMP_REQUIRE(max_len <= (1 << 30), SIMP_ERR_SHAPE, "attn_kv8: max_len %lld exceeds 2^30", (long long)max_len);
   if (n_seqs == 0) return SIMP_OK;
   SIMP_REQUIRE(n_seqs <= 65535, SIMP_ERR_SHAPE, "attn_kv8: more than 65535 sequences");
   SIMP_REQUIRE(q_dev && out_dev && lengths_dev, SIMP_ERR_ARG, "attn_kv8: null pointer");
@@ -880,6 +881,7 @@ SIMP_API int simp_gpu_attn_kv8(const simp_kv8_cache* cache, const int32_t* block
   const int nh = a.rep > 4 ? 2 : 1;
   const int64_t groups = int64_t(a.c.G) * ((a.rep + 4 * nh - 1) / (4 * nh));
   const int64_t slots = n_seqs * groups;
+  SIMP_REQUIRE(groups <= 65535, SIMP_ERR_SHAPE, "attn_kv8: too many heads");
   // Chunks of at least a tile per warp.  One sequence: as many blocks as run at once (three per SM), for joining costs as
   // much as it gains beyond that (131072 tokens, 8 x 128: 56 us with 54 chunks, 67 with 109, 87 with 205).  Several, whose
   // lengths differ: twice as many and none longer than 2048 tokens, so that the longest does not end alone (64 sequences of
@@ -894,7 +896,6 @@ SIMP_API int simp_gpu_attn_kv8(const simp_kv8_cache* cache, const int32_t* block
     a.count = static_cast<int*>(scratch(size_t(slots) * 4, SCRATCH_KV8_COUNT, true));
     if (!a.count) return scratch_failed("attn_kv8");
   }
-  SIMP_REQUIRE(groups <= 65535, SIMP_ERR_SHAPE, "attn_kv8: too many heads");
   const dim3 grid(unsigned(a.max_chunks), unsigned(groups), unsigned(n_seqs));
   cudaStream_t st = ctx().stream;
   const bool wide = dtype == SIMP_DTYPE_F32;

@@ -95,6 +95,7 @@ def test_attn_kv8(sg):
     refused(sg, SHAPE, "heads", fn, c, P, 4, P, P, P, 1, 8, 3)
     refused(sg, SHAPE, "heads", fn, c, P, 4, P, P, P, 1, 8, 0)
     refused(sg, SHAPE, "max_len", fn, c, P, 4, P, P, P, 1, 65, 4)
+    refused(sg, SHAPE, "2.30", fn, c, P, (1 << 27) - 1, P, P, P, 1, (1 << 30) + 1, 4)
     refused(sg, SHAPE, "65535", fn, c, P, 4, P, P, P, 70000, 8, 4)
     for hole in range(3):
         a = [P] * 3
