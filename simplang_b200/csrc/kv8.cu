@@ -116,11 +116,12 @@ __device__ __forceinline__ bool kv8_span(const Kv8View& c, int64_t unit, const i
   return true;
 }
 
-// A thread owns a patch of 16 tokens x 4 elements of K and the same of V: K leaves as words (a warp writes whole rows), V
-// as 16-byte columns.  A block of threads per (sequence, cache block, head): bt / 16 x pitch / 4 patches.  Rows are read
-// twice, for the maximum and for the values; the second time they come from L1.  (Keeping both patches in registers
-// between the passes was tried: 254 registers, and code so long that fetching it took most of the time; 8192 rows of 8
-// heads x 128 took 90 us, one token for each of 48 sequences 39.)
+// A thread owns a patch of 16 tokens x 4 elements of K or of V: K leaves as words (a warp writes whole rows), V as 16-byte
+// columns.  A block of threads per (sequence, cache block, head), for K and for V: bt / 16 x pitch / 4 patches.  Rows are
+// read twice, for the maximum and for the values; the second time most come from L1.  Bound by these round trips: a call
+// is hardly more than one wave of blocks (8192 bf16 rows of 8 heads x 128: 21 us, of 8 at the memory's rate; 26 with one
+// block for K and V, 23 with 4 rows of the first pass in flight, 21 with 16).  Keeping patches in registers between the
+// passes was tried: 254 registers, and code so long that fetching it took most of the time; 90 us.
 // VEC: four elements lie together at a multiple of their size (head_dim a multiple of 4, aligned pointers and stride).
 // Four elements as they are stored: what the maximum is taken of, two 16-bit ones at a time.
 template <typename T> struct Kv8Raw;
@@ -185,78 +186,65 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8View c, const T* __restrict__ k, const T* __restrict__ v,
                                                          int64_t row_stride, const int32_t* __restrict__ off,
                                                          const int32_t* __restrict__ starts, int n_seqs, int64_t total, int* status) {
-  __shared__ float tops[2][8];
+  __shared__ float tops[8];
   Kv8Span sp;
   pdl_launch_dependents();
   pdl_wait();
   if (!kv8_span(c, blockIdx.x, off, starts, n_seqs, total, status, sp)) return;
+  const bool is_v = blockIdx.z;
   const int h = blockIdx.y, quads = c.pitch >> 2, g = threadIdx.x / quads, d = 4 * (threadIdx.x % quads);
   const int t0 = 16 * g, lo = max(sp.a - t0, 0), hi = g < (c.bt >> 4) ? min(sp.b - t0, 16) : 0;   // new tokens of the patch: [lo, hi)
-  const int64_t at = (int64_t(sp.row0) + t0 - sp.a) * row_stride + int64_t(h) * c.D;
   const bool some = d < c.D;   // pad elements are written as zeros
-  const T *kr = k + at, *vr = v + at;
+  const T* in = (is_v ? v : k) + (int64_t(sp.row0) + t0 - sp.a) * row_stride + int64_t(h) * c.D;
   const int64_t sc = int64_t(sp.block) * c.G + h;
-  const float old_k = sp.a ? c.ks[sc] : 0.0f, old_v = sp.a ? c.vs[sc] : 0.0f;
-  uint32_t tk = 0, tv = 0;
-  if (some) {
-#pragma unroll 4
-    for (int j = lo; j < hi; ++j) {
-      kv8_raw4<T, VEC>(kr + j * row_stride, d, c.D).top(tk);
-      kv8_raw4<T, VEC>(vr + j * row_stride, d, c.D).top(tv);
-    }
+  float* scale = (is_v ? c.vs : c.ks) + sc;
+  const float old = sp.a ? *scale : 0.0f;
+  uint32_t t = 0;
+  if (some && lo == 0 && hi == 16) {
+#pragma unroll 8
+    for (int j = 0; j < 16; ++j) kv8_raw4<T, VEC>(in + j * row_stride, d, c.D).top(t);
+  } else if (some) {
+#pragma unroll 1
+    for (int j = lo; j < hi; ++j) kv8_raw4<T, VEC>(in + j * row_stride, d, c.D).top(t);
   }
-  float topk = Kv8Raw<T>::magnitude(tk), topv = Kv8Raw<T>::magnitude(tv);
-  const bool odd = __syncthreads_or(!(topk <= FLT_MAX) || !(topv <= FLT_MAX));
+  float top = Kv8Raw<T>::magnitude(t);
+  const bool odd = __syncthreads_or(!(top <= FLT_MAX));
   if (odd) {   // infinities and NaN do not count
-    topk = topv = 0.0f;
+    top = 0.0f;
 #pragma unroll 1
     for (int j = lo; some && j < hi; ++j) {
-      float x[4], y[4];
-      kv8_load4<T, VEC>(kr + j * row_stride, d, c.D, x);
-      kv8_load4<T, VEC>(vr + j * row_stride, d, c.D, y);
+      float x[4];
+      kv8_load4<T, VEC>(in + j * row_stride, d, c.D, x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        topk = fmaxf(topk, kv8_magnitude(x[i]));
-        topv = fmaxf(topv, kv8_magnitude(y[i]));
-      }
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, kv8_magnitude(x[i]));
     }
   }
-  topk = warp_max(topk);
-  topv = warp_max(topv);
-  if ((threadIdx.x & 31) == 0) {
-    tops[0][threadIdx.x >> 5] = topk;
-    tops[1][threadIdx.x >> 5] = topv;
-  }
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
   __syncthreads();
-  for (int i = 0; i < int(blockDim.x >> 5); ++i) {
-    topk = fmaxf(topk, tops[0][i]);
-    topv = fmaxf(topv, tops[1][i]);
-  }
-  const float sk = fmaxf(kv8_step(topk), old_k), sv = fmaxf(kv8_step(topv), old_v);
-  if (threadIdx.x == 0) {   // every thread has read the old scales: they were loaded before the barrier
-    c.ks[sc] = sk;
-    c.vs[sc] = sv;
-  }
-  const bool grew_k = sp.a && sk != old_k, grew_v = sp.a && sv != old_v;
+  for (int i = 0; i < int(blockDim.x >> 5); ++i) top = fmaxf(top, tops[i]);
+  const float s = fmaxf(kv8_step(top), old);
+  if (threadIdx.x == 0) *scale = s;   // every thread has read the old one: it was loaded before the barrier
   if (g >= (c.bt >> 4)) return;
-  const float ik = sk > 0.0f ? 1.0f / sk : 0.0f, iv = sv > 0.0f ? 1.0f / sv : 0.0f;
-  const float sure_k = kv8_sure(sk), sure_v = kv8_sure(sv);
-  int8_t* kb = c.k + sc * c.bt * c.pitch + int64_t(t0) * c.pitch + d;
-  int8_t* vb = c.v + sc * c.bt * c.pitch + (int64_t(g) * c.pitch + d) * 16;
-  const int held = min(lo, 16);   // tokens of the patch that the block held before
-  if (grew_k)
+  const float inv = s > 0.0f ? 1.0f / s : 0.0f, sure = kv8_sure(s);
+  const bool general = odd || s == 0.0f;
+  int8_t* to = (is_v ? c.v : c.k) + sc * c.bt * c.pitch + (is_v ? (int64_t(g) * c.pitch + d) * 16 : int64_t(t0) * c.pitch + d);
+  if (sp.a && s != old) {   // tokens of the patch that the block held before, to the larger step
+    const int per_token = is_v ? 1 : c.pitch, per_element = is_v ? 16 : 1;
 #pragma unroll 1
-    for (int i = 0; i < 4 * held; ++i) kb[(i >> 2) * c.pitch + (i & 3)] = int8_t(kv8_requantise(kb[(i >> 2) * c.pitch + (i & 3)], old_k, sk));
-  if (grew_v)
-#pragma unroll 1
-    for (int i = 0; i < 4 * held; ++i) vb[16 * (i & 3) + (i >> 2)] = int8_t(kv8_requantise(vb[16 * (i & 3) + (i >> 2)], old_v, sv));
-#pragma unroll 4
-  for (int j = lo; j < hi; ++j) {
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (some) kv8_load4<T, VEC>(kr + j * row_stride, d, c.D, x);
-    *reinterpret_cast<uint32_t*>(kb + j * c.pitch) = kv8_round4(x, sk, ik, sure_k, odd || sk == 0.0f);
+    for (int i = 0; i < 4 * min(lo, 16); ++i) {
+      int8_t& q = to[(i >> 2) * per_token + (i & 3) * per_element];
+      q = int8_t(kv8_requantise(q, old, s));
+    }
   }
-  if (lo == 0 && hi == 16) {
+  if (!is_v) {
+#pragma unroll 4
+    for (int j = lo; j < hi; ++j) {
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (some) kv8_load4<T, VEC>(in + j * row_stride, d, c.D, x);
+      *reinterpret_cast<uint32_t*>(to + j * c.pitch) = kv8_round4(x, s, inv, sure, general);
+    }
+  } else if (lo == 0 && hi == 16) {
     uint32_t col[4][4];   // element, four words of four tokens
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -264,8 +252,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8View c, const T* __r
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (some) kv8_load4<T, VEC>(vr + (4 * w + j) * row_stride, d, c.D, x);
-        r[j] = kv8_round4(x, sv, iv, sure_v, odd || sv == 0.0f);
+        if (some) kv8_load4<T, VEC>(in + (4 * w + j) * row_stride, d, c.D, x);
+        r[j] = kv8_round4(x, s, inv, sure, general);
       }
       // rows of four elements to columns of four tokens
       const uint32_t p0 = __byte_perm(r[0], r[1], 0x5140), p1 = __byte_perm(r[0], r[1], 0x7362);
@@ -276,15 +264,15 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8View c, const T* __r
       col[3][w] = __byte_perm(p1, q1, 0x7632);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(vb)[i] = make_uint4(col[i][0], col[i][1], col[i][2], col[i][3]);
+    for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(col[i][0], col[i][1], col[i][2], col[i][3]);
   } else {   // part of a column: byte by byte, what lies before and behind the new tokens stays
 #pragma unroll 1
     for (int j = lo; j < hi; ++j) {
       float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (some) kv8_load4<T, VEC>(vr + j * row_stride, d, c.D, x);
-      const uint32_t r = kv8_round4(x, sv, iv, sure_v, odd || sv == 0.0f);
+      if (some) kv8_load4<T, VEC>(in + j * row_stride, d, c.D, x);
+      const uint32_t r = kv8_round4(x, s, inv, sure, general);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vb[16 * i + j] = int8_t(r >> (8 * i));
+      for (int i = 0; i < 4; ++i) to[16 * i + j] = int8_t(r >> (8 * i));
     }
   }
 }
@@ -298,31 +286,40 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8View c, T* __restrict_
   pdl_launch_dependents();
   pdl_wait();
   if (!kv8_span(c, blockIdx.x, off, starts, n_seqs, total, status, sp)) return;
+  const bool is_v = blockIdx.z;
   const int h = blockIdx.y, quads = c.pitch >> 2, g = threadIdx.x / quads, d = 4 * (threadIdx.x % quads);
   const int t0 = 16 * g, lo = max(sp.a - t0, 0), hi = g < (c.bt >> 4) ? min(sp.b - t0, 16) : 0;
   if (hi <= lo || d >= c.D) return;
   const int64_t sc = int64_t(sp.block) * c.G + h;
-  const float sk = __ldg(c.ks + sc), sv = __ldg(c.vs + sc);
-  const int8_t* kb = c.k + sc * c.bt * c.pitch + int64_t(t0) * c.pitch + d;
-  const uint4* vb = reinterpret_cast<const uint4*>(c.v + sc * c.bt * c.pitch) + int64_t(g) * c.pitch + d;
-  uint32_t kw[16];
+  const float s = __ldg((is_v ? c.vs : c.ks) + sc);
+  T* out = (is_v ? v : k) + (int64_t(sp.row0) + t0 - sp.a) * row_stride + int64_t(h) * c.D;
+  uint32_t w[16];   // four elements of token 4 t + j in word 4 j + t
+  if (!is_v) {
+    const int8_t* kb = c.k + (sc * c.bt + t0) * c.pitch + d;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) kw[j] = __ldcs(reinterpret_cast<const uint32_t*>(kb + j * c.pitch));
-  uint4 vw[4];
+    for (int j = 0; j < 16; ++j) w[4 * (j & 3) + (j >> 2)] = __ldcs(reinterpret_cast<const uint32_t*>(kb + j * c.pitch));
+  } else {
+    const uint4* vb = reinterpret_cast<const uint4*>(c.v + sc * c.bt * c.pitch) + int64_t(g) * c.pitch + d;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) vw[i] = __ldcs(vb + i);
-  const int64_t at = (int64_t(sp.row0) + t0 - sp.a) * row_stride + int64_t(h) * c.D;
-  auto byte_of = [](uint32_t w, int i) { return float(int8_t(uint8_t(w >> (8 * i)))); };
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = __ldcs(vb + i);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {   // columns of four tokens to rows of four elements
+      const uint32_t p0 = __byte_perm(w[t], w[4 + t], 0x5140), p1 = __byte_perm(w[t], w[4 + t], 0x7362);
+      const uint32_t q0 = __byte_perm(w[8 + t], w[12 + t], 0x5140), q1 = __byte_perm(w[8 + t], w[12 + t], 0x7362);
+      w[t] = __byte_perm(p0, q0, 0x5410);
+      w[4 + t] = __byte_perm(p0, q0, 0x7632);
+      w[8 + t] = __byte_perm(p1, q1, 0x5410);
+      w[12 + t] = __byte_perm(p1, q1, 0x7632);
+    }
+  }
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     if (j < lo || j >= hi) continue;
+    const uint32_t r = w[4 * (j & 3) + (j >> 2)];
     float x[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = byte_of(kw[j], i) * sk;
-    kv8_store4<T, VEC>(k + at + j * row_stride, d, c.D, x);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = byte_of((&vw[i].x)[j >> 2], j & 3) * sv;
-    kv8_store4<T, VEC>(v + at + j * row_stride, d, c.D, x);
+    for (int i = 0; i < 4; ++i) x[i] = float(int8_t(uint8_t(r >> (8 * i)))) * s;
+    kv8_store4<T, VEC>(out + j * row_stride, d, c.D, x);
   }
 }
 
@@ -805,7 +802,7 @@ static int kv8_rows(const char* who, bool write, const simp_kv8_cache* cache, co
   DeviceScope dev;
   cudaStream_t st = ctx().stream;
   // a sequence of n rows touches at most (n - 1) / bt + 2 blocks, and never more than n
-  const dim3 grid(unsigned(std::min<int64_t>(total, total / c.bt + 2 * n_seqs)), unsigned(c.G));
+  const dim3 grid(unsigned(std::min<int64_t>(total, total / c.bt + 2 * n_seqs)), unsigned(c.G), 2);   // z: K, V
   int* status = ctx().dev_status;
   const unsigned threads = unsigned((c.bt / 16 * (c.pitch / 4) + 31) / 32 * 32);
   const size_t four = 4 * dtype_size(dtype);
