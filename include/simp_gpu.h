@@ -228,8 +228,8 @@ int simp_gpu_attn_kv8(const simp_kv8_cache* cache, const int32_t* block_table_de
  *   n > 0:  x = x > 0 ? x / repetition[r] : x * repetition[r];   x = x - (frequency[r] * n + presence[r])
  *   x = x + bias_values[e] for the LAST entry e of bias_offsets[r] .. with bias_tokens[e] == t
  *   bit t % 32 of word t / 32 of the row's mask is 0:  x = -infinity
- * n_tokens and n_bias are the lengths of the id lists; allowed_stride is the distance of the rows' masks in words
- * (at least ceil(vocab / 32)), 0: one mask for all rows. */
+ * n_tokens and n_bias are the lengths of the id lists (at most 2^30); allowed_stride is the distance of the rows' masks in
+ * words (at least ceil(vocab / 32)), 0: one mask for all rows. */
 typedef struct simp_logits_rules {
   const int32_t* tokens;
   const int32_t* token_offsets; /* [rows + 1] */

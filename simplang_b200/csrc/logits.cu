@@ -73,8 +73,7 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
     }
   };
   load(0, x[0], mlo[0], mhi[0]);
-  // ---- the few: `changed` holds a token's last bias entry, then how often it stands in the history, then its new logit,
-  // which a bit announces.  Loads of a step are issued together; each step is a round trip to L2 at most.
+  // ---- the few: `changed` holds how often a token stands in the history, then its new logit, which a bit announces.  Loads of a step are issued together; each step is a round trip to L2 at most.
   int* changed = lg_smem;                                             // [SLICE]
   uint32_t* bits = reinterpret_cast<uint32_t*>(lg_smem + SLICE);      // [SLICE / 32]
   uint32_t* biased = bits + SLICE / 32;                               // [SLICE / 32]
@@ -94,30 +93,27 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
       }
     };
     fetch(hb);
+    const int bias0 = a.r.bias_tokens && bb + tid < be ? __ldg(a.r.bias_tokens + bb + tid) : -1;
     for (int i = 4 * tid; i < SLICE + SLICE / 16; i += 4 * LG_THREADS) *reinterpret_cast<int4*>(lg_smem + i) = make_int4(0, 0, 0, 0);
     const float rep = a.r.repetition ? __ldg(a.r.repetition + row) : 1.0f;
     const float freq = a.r.frequency ? __ldg(a.r.frequency + row) : 0.0f;
     const float pres = a.r.presence ? __ldg(a.r.presence + row) : 0.0f;
+    // their logits on the way to L2
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+      if (ids[k] >= 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(in + base + ids[k]));
+    if (bias0 >= first && bias0 < last) asm volatile("prefetch.global.L2 [%0];" ::"l"(in + bias0));
     __syncthreads();
-    // Biases: the last entry of a token counts.  Up to 32 entries per thread are compared in `changed`, which is zero before
-    // and after, and a thread keeps which of its entries count in a word; longer lists are walked by one warp, below.
-    const int n_bias = be - bb, per = n_bias <= 32 * LG_THREADS ? (n_bias + LG_THREADS - 1) / LG_THREADS : 0;
-    uint32_t won = 0;
     auto entry = [&](int i) {   // place in the slice of a bias entry's token, or -1
       const int id = i >= bb && i < be ? __ldg(a.r.bias_tokens + i) : -1;
       return id >= first && id < last ? id - base : -1;
     };
-    if (per > 0) {
-      for (int k = 0; k < per; ++k)
-        if (const int i = k * LG_THREADS + tid, at = entry(bb + i); at >= 0) atomicMax(changed + at, i + 1);
-      __syncthreads();
-      for (int k = 0; k < per; ++k)
-        if (const int i = k * LG_THREADS + tid, at = entry(bb + i); at >= 0 && changed[at] == i + 1) won |= 1u << k;
-      __syncthreads();
-      for (int k = 0; k < per; ++k)
-        if ((won >> k) & 1u) changed[entry(bb + k * LG_THREADS + tid)] = 0;
-      __syncthreads();
-    }
+    bool twice = false;   // a token stands twice among the biases: rare, and its last entry counts
+    for (int i = bb + tid; i < be; i += LG_THREADS)
+      if (const int at = entry(i); at >= 0) {
+        const uint32_t bit = 1u << (at & 31);
+        twice = twice || (atomicOr(biased + (at >> 5), bit) & bit);
+      }
     if (he > hb) {
       for (int i0 = hb;;) {
 #pragma unroll
@@ -127,7 +123,9 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
         if (i0 >= he) break;
         fetch(i0);
       }
-      __syncthreads();
+    }
+    twice = __syncthreads_or(twice);
+    if (he > hb) {
       for (int i0 = hb;;) {
         if (he - hb > E * LG_THREADS) fetch(i0);
         float v[E];
@@ -157,10 +155,12 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
       const bool held = atomicOr(bits + (at >> 5), bit) & bit;
       changed[at] = __float_as_int(__fadd_rn(held ? __int_as_float(changed[at]) : raw, value));
     };
-    if (per > 0) {
-      for (int k = 0; k < per; ++k)
-        if ((won >> k) & 1u) add(bb + k * LG_THREADS + tid, entry(bb + k * LG_THREADS + tid));
+    if (!twice) {
+      for (int i = bb + tid; i < be; i += LG_THREADS)
+        if (const int at = entry(i); at >= 0) add(i, at);
     } else if (tid < 32) {
+      for (int w = lane; w < SLICE / 32; w += 32) biased[w] = 0u;
+      __syncwarp();
       for (int i0 = be; i0 > bb; i0 -= 32) {   // from the last entry to the first: a token that is marked has had its own
         const int i = i0 - 1 - lane, at = entry(i);
         const unsigned same = __match_any_sync(0xffffffffu, at >= 0 ? at : -1 - lane);
@@ -264,7 +264,7 @@ static int logits_run(LogitsArgs& a) {
 }
 
 // Slices of 8192 tokens where that still gives every SM two blocks, else of 1024 (f32) or 2048.  200 rows of 128256 with
-// histories of 2000: 61 us with 8192, 73 with 16384 (three blocks per SM), 86 with 4096 (histories read twice as often);
+// histories of 2000: 57 us with 8192, 64 with 16384 (three blocks per SM), 76 with 4096 (histories read twice as often);
 // without history and biases 36 us, 0.87 of the memory's rate.
 template <typename T>
 static int logits_launch(LogitsArgs& a) {
@@ -294,7 +294,8 @@ SIMP_API int simp_gpu_logits_process(const void* logits_dev, void* out_dev, int6
   SIMP_REQUIRE(r.tokens || !(r.repetition || r.frequency || r.presence), SIMP_ERR_ARG, "logits_process: penalties need tokens");
   SIMP_REQUIRE((r.bias_tokens != nullptr) == (r.bias_values != nullptr) && (r.bias_tokens != nullptr) == (r.bias_offsets != nullptr),
                SIMP_ERR_ARG, "logits_process: bias_tokens, bias_values and bias_offsets go together");
-  SIMP_REQUIRE(r.n_tokens >= 0 && r.n_tokens <= INT_MAX && r.n_bias >= 0 && r.n_bias <= INT_MAX, SIMP_ERR_ARG, "logits_process: bad length of a list");
+  SIMP_REQUIRE(r.n_tokens >= 0 && r.n_tokens <= (1 << 30) && r.n_bias >= 0 && r.n_bias <= (1 << 30), SIMP_ERR_ARG,
+               "logits_process: a list's length is outside 0 .. 2^30");
   SIMP_REQUIRE(!r.allowed || r.allowed_stride == 0 || r.allowed_stride >= (vocab + 31) / 32, SIMP_ERR_SHAPE,
                "logits_process: allowed_stride %lld words for %lld tokens", (long long)r.allowed_stride, (long long)vocab);
   if (int rc = ensure_ready()) return rc;

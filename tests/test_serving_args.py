@@ -125,6 +125,12 @@ def test_logits_process(sg):
     refused(sg, SHAPE, "allowed_stride", fn, P, P, 1, 33, r(allowed=P, allowed_stride=1))
 
 
+def test_lists_longer_than_the_kernel_counts(sg):
+    fn, r, n = sg.logits_process, sg.logits_rules, (1 << 30) + 1
+    refused(sg, ARG, "list", fn, P, P, 1, 8, r(tokens=P, token_offsets=P, n_tokens=n))
+    refused(sg, ARG, "list", fn, P, P, 1, 8, r(bias_tokens=P, bias_values=P, bias_offsets=P, n_bias=n))
+
+
 def test_sizes_of_a_cache(sg):
     assert sg.kv8_bytes(10, 16, 2, 100) == (10 * 16 * 2 * 128, 10 * 16 * 2 * 128, 80, 80)
     assert C.sizeof(sg.Kv8Cache) == 64 and C.sizeof(sg.LogitsRules) == 96
