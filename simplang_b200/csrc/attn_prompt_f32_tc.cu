@@ -6,13 +6,19 @@
 // size, and (2) the output of every tile of keys is a sum of its own, added to f32 registers with rounding: an
 // accumulator kept over a long prompt would drift by 2e-8 per instruction.
 //
-// One block of 12 warps per row tile (128 rows: 128 / rep tokens x the rep heads that share a key/value head):
-//   warp 0      TMA: the planes of K and V per tile of 64 keys (head sizes up to 64: 128), two stages of 48 KB each
-//   warp 1      MMAs: S = Q K^T as soon as the softmax has read the S before; T = P V into a TMEM tile
-//   warps 4-11  softmax, two threads per row; P in three planes to TMEM; T into registers (D / 2 each)
-// The planes of Q lie in TMEM: from shared memory they would be read again for every product (6 KB per MMA of 32 cycles,
-// where shared memory gives 128 bytes a cycle: 77 cycles were measured), and there would be no room for second stages.
-// Per tile the tensor cores need 3072 cycles, the softmax about as many beside them.
+// One block of 18 warps per row tile (128 rows: 128 / rep tokens x the rep heads that share a key/value head):
+//   warp 0      TMA: the planes of K and V per tile of 128 keys (96 KB each for head sizes above 64)
+//   warp 1      MMAs: S = Q K^T, then T = P V, into TMEM
+//   warps 2-17  softmax, four threads per row; P in three planes to TMEM; T into registers (D / 4 each)
+// The planes of Q lie in TMEM, where they take no shared memory (and are not read from it again for every product: 6 KB per
+// MMA of 64 keys, where it gives 128 bytes a cycle).  That leaves no TMEM for a second S, so P replaces S and softmax and
+// MMAs take turns; only T is added up while the next scores are multiplied.  The form before had tiles of 64 keys, whose S
+// and P lay apart, and overlapped the two: an MMA of 64 keys takes no less time than one of 96 (50 cycles, 75 beside the
+// softmax), so it lost more than it won (4 prompts of 2048, 32 heads of 128: 1180 us, now 1020; of 100: 1265, now 985).
+// A step of 128 keys takes 10700 cycles: 4200 S (48 MMAs, 64 cycles each when nothing loads), 2650 softmax (1024 of them
+// exponentials), 3100 T, the rest hand-overs.  Loading V later, when no MMA runs, costs more than it gives (1085 us).
+// Head sizes up to 64 have half the MMAs for S and keep T apart for each plane of V, which lets one MMA multiply a plane of P
+// with up to three planes of V side by side (25 MMAs of up to 192 columns instead of 48 of 64, which take no less than 96).
 //
 // No plane product of an infinity or a NaN is right, and a zero weight does not hide them from an MMA (a tile may hold keys
 // that some rows must not see, or rows of the next sequence).  The splitting pass leaves them out of the planes and marks
@@ -25,17 +31,24 @@
 
 namespace simp {
 
-constexpr int F3_THREADS = 384;
+constexpr int F3_THREADS = 576;   // (five warps on some scheduler: 96 registers a thread)
 
 template <int D>
 struct F3Shape {
-  static constexpr int KEYS = D == 64 ? 128 : 64, ATOM = KEYS * 128;   // bytes of 64 elements of a tile's rows
+  static constexpr int KEYS = 128, ATOM = KEYS * 128;   // bytes of 64 elements of a tile's rows
   static constexpr int PLANE = KEYS * D * 2, STAGE = 3 * PLANE;
-  static constexpr int BARS = 13;
-  static constexpr size_t SMEM = 4 * size_t(STAGE) + BARS * 8 + 16 + 8 * 128 + 24;
-  static constexpr uint32_t P = KEYS, T = P + 3 * KEYS / 2, Q = T + D;   // TMEM columns: S, three planes of P, T, three planes of Q
+  static constexpr int BARS = 8;
+  static constexpr size_t SMEM = 2 * size_t(STAGE) + BARS * 8 + 16 + 16 * 128 + 24;
+  // TMEM columns: S, which the planes of P replace (192: see place_of_p), T (head sizes up to 64: three), three planes of Q
+  static constexpr uint32_t T = 192, Q = T + (D == 64 ? 3 * 64 : 128);
   static_assert(Q + 3 * D / 2 <= 512 && SMEM <= 232448, "");
 };
+// TMEM columns of P for 16 keys (step 0 .. 7 of a tile) and a plane.  S is 128 columns, P 192: a thread that takes the scores
+// of its 32 keys frees 32 columns for 48 that it writes, and touches no column of the row's other threads.
+__host__ __device__ constexpr uint32_t place_of_p(int step, int plane) {
+  const int part = step >> 1, b = 3 * (step & 1) + plane;
+  return b < 2 ? 128u + 16u * part + 8u * b : 32u * part + 8u * (b - 2);
+}
 
 struct F3Args {
   AttnPromptArgs a;
@@ -56,19 +69,16 @@ template <int D>
 __global__ void __launch_bounds__(F3_THREADS, 1)
     attn_prompt_f32_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const F3Args p) {
   using Sh = F3Shape<D>;
-  constexpr int KEYS = Sh::KEYS, MINE = KEYS / 2;   // keys of a tile, of a thread
+  constexpr int KEYS = Sh::KEYS, MINE = 32;   // keys of a tile, of a thread
   extern __shared__ __align__(1024) uint8_t f3_raw[];
-  const uint32_t base = smem_u32(f3_raw), k_smem = base, v_smem = base + 2 * Sh::STAGE, bars = base + 4 * Sh::STAGE;
-  auto k_full = [&](int s) { return bars + 8u * s; };
-  auto k_empty = [&](int s) { return bars + 16u + 8u * s; };
-  auto v_full = [&](int s) { return bars + 32u + 8u * s; };
-  auto v_empty = [&](int s) { return bars + 48u + 8u * s; };
-  const uint32_t s_bar = bars + 64, s_read = bars + 72, p_bar = bars + 80, t_bar = bars + 88, q_bar = bars + 96;
-  uint8_t* tail = f3_raw + 4 * Sh::STAGE + Sh::BARS * 8;
+  const uint32_t base = smem_u32(f3_raw), k_smem = base, v_smem = base + Sh::STAGE, bars = base + 2 * Sh::STAGE;
+  auto k_full = [&](int plane) { return bars + 8u * plane; };
+  const uint32_t v_full = bars + 24, s_bar = bars + 32, p_bar = bars + 40, t_bar = bars + 48, q_bar = bars + 56;
+  uint8_t* tail = f3_raw + 2 * Sh::STAGE + Sh::BARS * 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8);
-  float* half_row = reinterpret_cast<float*>(tail + 16);   // [half][row]
-  volatile int* found_unit = reinterpret_cast<volatile int*>(half_row + 2 * 128);   // found, place, q0, q1, k0, k1
+  float* part_row = reinterpret_cast<float*>(tail + 16);   // [part][row]
+  volatile int* found_unit = reinterpret_cast<volatile int*>(part_row + 4 * 128);   // found, place, q0, q1, k0, k1
   const AttnPromptArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {   // never: the declaration asks for it
@@ -76,17 +86,12 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
     return;
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(k_full(i), 1);
-      mbar_init(k_empty(i), 1);
-      mbar_init(v_full(i), 1);
-      mbar_init(v_empty(i), 1);
-    }
+    for (int i = 0; i < 3; ++i) mbar_init(k_full(i), 1);
+    mbar_init(v_full, 1);
     mbar_init(s_bar, 1);
-    mbar_init(s_read, 8);
-    mbar_init(p_bar, 8);
+    mbar_init(p_bar, 16);
     mbar_init(t_bar, 1);
-    mbar_init(q_bar, 8);
+    mbar_init(q_bar, 16);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -137,23 +142,31 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
   const int r0 = ((nq + p.tpt - 1) / p.tpt - 1 - place) * p.tpt;   // the longest rows first
   const int64_t shift = int64_t(nk) - nq;
   auto sees = [&](int token) { return int(max(int64_t(0), min(int64_t(nk), token + shift + 1))); };
-  const int n = (sees(min(r0 + p.tpt, nq) - 1) + KEYS - 1) / KEYS;
+  const int keys = sees(min(r0 + p.tpt, nq) - 1), n = (keys + KEYS - 1) / KEYS;
+  auto steps = [&](int j) { return min(KEYS, keys - KEYS * j + 15) >> 4; };   // of 16 keys in tile j that some row sees
 
   if (warp == 0) {
     // ------------------------------------------------------------------ loads
     if (lane == 0 && n > 0) {
       bool ok = true;
-      auto tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, uint32_t empty, int j) {
-        ok = ok && wait_bar(empty, ((j >> 1) & 1) ^ 1, abort_flag, a.status, 71);
-        if (!ok) return;
-        mbar_arrive_expect_tx(full, Sh::STAGE);
-        for (int s = 0; s < 3; ++s)
-          for (int b = 0; b < D / 64; ++b)
-            tma_load_3d(dst + (j & 1) * Sh::STAGE + s * Sh::PLANE + b * Sh::ATOM, map, full, 64 * b, g, int(s * a.total_k) + k0 + KEYS * j);
+      auto boxes = [&](int j) { return steps(j) > 4 ? 2 : 1; };   // of 64 keys
+      auto plane = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int s, int j) {
+        for (int b = 0; b < D / 64; ++b)
+          for (int i = 0; i < boxes(j); ++i)
+            tma_load_3d(dst + s * Sh::PLANE + b * Sh::ATOM + i * (Sh::ATOM / 2), map, full, 64 * b, g, int(s * a.total_k) + k0 + KEYS * j + 64 * i);
       };
       for (int j = 0; ok && j < n; ++j) {
-        tile(&map_k, k_smem, k_full(j & 1), k_empty(j & 1), j);
-        tile(&map_v, v_smem, v_full(j & 1), v_empty(j & 1), j);
+        ok = j == 0 || wait_bar(s_bar, (j - 1) & 1, abort_flag, a.status, 71);
+        if (!ok) break;
+        for (int i = 0; i < 3; ++i) {
+          const int s = i == 0 ? 0 : 3 - i;   // as the products need them
+          mbar_arrive_expect_tx(k_full(s), boxes(j) * (Sh::PLANE / 2));
+          plane(&map_k, k_smem, k_full(s), s, j);
+        }
+        ok = j == 0 || wait_bar(t_bar, (j - 1) & 1, abort_flag, a.status, 81);
+        if (!ok) break;
+        mbar_arrive_expect_tx(v_full, boxes(j) * (Sh::STAGE / 2));
+        for (int s = 0; s < 3; ++s) plane(&map_v, v_smem, v_full, s, j);
       }
       if (!ok)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);   // let copies in flight land before the block retires
@@ -161,9 +174,7 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMAs (the whole warp with the same values, one lane issues)
-    constexpr uint32_t idesc_s = idesc_f16(true, KEYS, false);
-    const int width = (a.D + 15) / 16;                        // steps of 16 elements that hold something
-    const uint32_t idesc_t = idesc_f16(true, 16 * width, true);
+    const int width = (a.D + 15) / 16;   // steps of 16 elements that hold something
     const bool leader = lane == 0;
     auto wait = [&](uint32_t bar, uint32_t phase, int site) {
       const bool ok = __all_sync(0xffffffffu, wait_bar(bar, phase, abort_flag, a.status, site));
@@ -173,75 +184,76 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
     // planes of the two operands, small products first
     constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
     auto scores = [&](int j) {
-      const uint64_t kd = make_smem_desc_sw128(k_smem, 16u, 1024u) + uint64_t((j & 1) * (Sh::STAGE / 16));
+      const uint32_t idesc = idesc_f16(true, 16 * steps(j), false);
+      const uint64_t kd = make_smem_desc_sw128(k_smem, 16u, 1024u);
 #pragma unroll
-      for (int t = 0; t < 6; ++t)
+      for (int t = 0; t < 6; ++t) {
+        if (j == 0 && t < 3 && !wait(k_full(PB[t]), 0, 73)) return false;   // (later ones have been waited for)
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-          mma_f16_ts(tmem, tmem + Sh::Q + uint32_t(D / 2) * PA[t] + 8u * s, kd + uint64_t(PB[t] * (Sh::PLANE / 16) + (s >> 2) * (Sh::ATOM / 16) + (s & 3) * 2),
-                     idesc_s, t > 0 || s > 0, leader && s < width);
+          if (s < D / 32 || s < width)   // (an MMA that is not issued still costs its instructions, about as much as one that is)
+            mma_f16_ts(tmem, tmem + Sh::Q + uint32_t(D / 2) * PA[t] + 8u * s, kd + uint64_t(PB[t] * (Sh::PLANE / 16) + (s >> 2) * (Sh::ATOM / 16) + (s & 3) * 2),
+                       idesc, t > 0 || s > 0, leader);
+      }
+      if (leader) mma_commit(s_bar);
+      return true;
+    };
+    const uint64_t vd = make_smem_desc_sw128(v_smem, uint32_t(Sh::ATOM), 1024u);   // [key][element]: 8 keys 1 KB apart
+    auto product = [&](int step, int pa, int pb, uint32_t idesc, bool acc, bool issue) {   // P plane pa, V planes pb ..
+      mma_f16_ts(tmem + Sh::T + (D == 64 ? 64u * pb : 0u), tmem + place_of_p(step, pa), vd + uint64_t(pb * (Sh::PLANE / 16) + step * 128), idesc, acc, leader && issue);
     };
     auto values = [&](int j) {
-      const uint64_t vd = make_smem_desc_sw128(v_smem, uint32_t(Sh::ATOM), 1024u) + uint64_t((j & 1) * (Sh::STAGE / 16));   // 8 keys 1 KB apart
+      const int have = steps(j);
+      if constexpr (D == 64) {   // planes of V side by side: what one plane of P is multiplied with takes one MMA
+        constexpr uint32_t ONE = idesc_f16(true, 64, true), TWO = idesc_f16(true, 128, true), ALL = idesc_f16(true, 192, true);
 #pragma unroll
-      for (int t = 0; t < 6; ++t)
+        for (int s = 0; s < 8; ++s) product(s, 1, 0, TWO, s > 0, s < have);
 #pragma unroll
-        for (int s = 0; s < KEYS / 16; ++s)
-          mma_f16_ts(tmem + Sh::T, tmem + Sh::P + uint32_t(KEYS / 2) * PA[t] + 8u * s, vd + uint64_t(PB[t] * (Sh::PLANE / 16) + s * 128), idesc_t, t > 0 || s > 0,
-                     leader);
+        for (int s = 0; s < 8; ++s) product(s, 2, 0, ONE, true, s < have);
+        product(0, 0, 2, ONE, false, true);   // begins the third sum
+        product(0, 0, 0, TWO, true, true);
+#pragma unroll
+        for (int s = 1; s < 8; ++s) product(s, 0, 0, ALL, true, s < have);
+      } else {
+        const uint32_t idesc = idesc_f16(true, 16 * width, true);
+#pragma unroll
+        for (int t = 0; t < 6; ++t)
+#pragma unroll
+          for (int s = 0; s < 8; ++s) product(s, PA[t], PB[t], idesc, t > 0 || s > 0, s < have);
+      }
+      if (leader) mma_commit(t_bar);
     };
-    bool ok = true;
-    if (n > 0) {
-      ok = wait(q_bar, 0, 72) && wait(k_full(0), 0, 73);
-      if (ok) {
-        scores(0);
-        if (leader) {
-          mma_commit(s_bar);
-          mma_commit(k_empty(0));
-        }
-      }
-    }
+    bool ok = n == 0 || wait(q_bar, 0, 72);
     for (int j = 0; ok && j < n; ++j) {
-      if (j + 1 < n) {
-        ok = wait(k_full((j + 1) & 1), ((j + 1) >> 1) & 1, 74) && wait(s_read, j & 1, 75);
-        if (!ok) break;
-        scores(j + 1);
-        if (leader) {
-          mma_commit(s_bar);
-          mma_commit(k_empty((j + 1) & 1));
-        }
-      }
-      ok = wait(v_full(j & 1), (j >> 1) & 1, 76) && wait(p_bar, j & 1, 77);
-      if (!ok) break;
-      values(j);
-      if (leader) {
-        mma_commit(t_bar);
-        mma_commit(v_empty(j & 1));
-      }
+      ok = scores(j);   // behind the products that read the P before: MMAs of one thread run in order
+      ok = ok && wait(v_full, j & 1, 76);
+      for (int s = 0; ok && j + 1 < n && s < 3; ++s) ok = wait(k_full(s), (j + 1) & 1, 74);   // here nothing waits for it
+      ok = ok && wait(p_bar, j & 1, 77);
+      if (ok) values(j);
     }
     if (!ok)
       for (int i = 0; i < 64; ++i) __nanosleep(1000);
     __syncwarp();
-  } else if (warp >= 4) {
+  } else {
     // ------------------------------------------------------------------ softmax and sums
-    const int half = (warp - 4) >> 2, row = threadIdx.x & 127;
+    const int part = (warp - 2) >> 2, row = 32 * (warp & 3) + lane;
     const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-    const uint32_t s_tmem = tmem + lanes + uint32_t(MINE) * half, t_tmem = tmem + Sh::T + lanes + uint32_t(D / 2) * half;
+    const uint32_t s_tmem = tmem + lanes + uint32_t(MINE) * part, t_tmem = tmem + Sh::T + lanes + uint32_t(D / 4) * part;
     const int token = r0 + row / a.rep, head = g * a.rep + row % a.rep;
     const bool mine = row < p.tpt * a.rep && token < nq;
     const int lim = mine ? sees(token) : 0;
-    volatile float* to = half_row + half * 128 + row;
-    volatile float* from = half_row + (half ^ 1) * 128 + row;
-    // this row's planes of Q, half a row per thread, to TMEM (rows behind the sequence: zeros)
+    volatile float* to = part_row + part * 128 + row;
+    volatile float* all = part_row + row;
+    // this row's planes of Q, a quarter of a row per thread, to TMEM (rows behind the sequence: zeros)
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t(q) * a.total_q + q0 + token) * a.H * D + int64_t(head) * D + (D / 2) * half);
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t(q) * a.total_q + q0 + token) * a.H * D + int64_t(head) * D + (D / 4) * part);
 #pragma unroll
-      for (int h = 0; h < D / 32; ++h) {   // 16 elements
+      for (int h = 0; h < D / 64; ++h) {   // 16 elements
         uint32_t w[8];
         const uint4 x = mine ? __ldg(src + 2 * h) : make_uint4(0u, 0u, 0u, 0u), y = mine ? __ldg(src + 2 * h + 1) : make_uint4(0u, 0u, 0u, 0u);
         w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
-        tmem_st_32x8(tmem + lanes + Sh::Q + uint32_t(D / 2) * q + uint32_t(D / 4) * half + 8u * h, w);
+        tmem_st_32x8(tmem + lanes + Sh::Q + uint32_t(D / 2) * q + uint32_t(D / 8) * part + 8u * h, w);
       }
     }
     tmem_st_wait();
@@ -249,27 +261,42 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
     __syncwarp();
     if (lane == 0) mbar_arrive(q_bar);
     const bool any = __ldcg(p.any) != 0, odd_row = any && mine && p.odd_q[int64_t(q0 + token) * a.H + head];
-    float m = -INFINITY, l = 0.0f, o[D / 2];
+    float m = -INFINITY, l = 0.0f, alpha = 0.0f, o[D / 4];
 #pragma unroll
-    for (int i = 0; i < D / 2; ++i) o[i] = 0.0f;
-    auto add_tile = [&](float alpha) {   // the tile's sum to the registers, then both to the new maximum
+    for (int i = 0; i < D / 4; ++i) o[i] = 0.0f;
+    auto add_tile = [&] {   // the sum of the last tile to the registers, which its maximum has not reached yet
 #pragma unroll
-      for (int h = 0; h < D / 32; ++h) {
+      for (int h = 0; h < D / 64; ++h) {
         uint32_t t[16];
         tmem_ld_32x16(t_tmem + 16u * h, t);
-        tmem_ld_wait();
+        if constexpr (D == 64) {
+          uint32_t t1[16], t2[16];
+          tmem_ld_32x16(t_tmem + 64u + 16u * h, t1);
+          tmem_ld_32x16(t_tmem + 128u + 16u * h, t2);
+          tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[16 * h + i] = (o[16 * h + i] + __uint_as_float(t[i])) * alpha;
+          for (int i = 0; i < 16; ++i) t[i] = __float_as_uint(__uint_as_float(t[i]) + (__uint_as_float(t1[i]) + __uint_as_float(t2[i])));
+        } else {
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[16 * h + i] = fmaf(o[16 * h + i], alpha, __uint_as_float(t[i]));
       }
     };
+    const f2 c2 = pack_f2(a.scale_log2, a.scale_log2), none = 0;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
+      if (j > 0) {   // while the scores are multiplied
+        ok = __all_sync(0xffffffffu, wait_bar(t_bar, (j - 1) & 1, abort_flag, a.status, 79)) && ok;
+        tc_fence_after_sync();
+        add_tile();
+      }
       ok = wait_bar(s_bar, j & 1, abort_flag, a.status, 78) && ok;
       tc_fence_after_sync();
       if (any) {   // rare: scores of rows that are not finite, by the f32 tensors
 #pragma unroll 1
         for (int i = 0; i < MINE; ++i) {
-          const int key = KEYS * j + MINE * half + i;
+          const int key = KEYS * j + MINE * part + i;
           uint32_t v = tmem_ld_1(s_tmem + i);
           tmem_ld_wait();
           if (key < lim && (odd_row || p.odd_k[int64_t(k0 + key) * a.G + g])) {
@@ -285,48 +312,59 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
         }
         tmem_st_wait();
       }
+      const int see = lim - KEYS * j - MINE * part, chunks = steps(j) - 2 * part;   // of 16 keys
+      const bool masked = __any_sync(0xffffffffu, see < MINE);
+      const int most = masked ? __reduce_max_sync(0xffffffffu, see) : MINE;   // keys behind it no row of the warp sees
+      float t[2] = {-INFINITY, -INFINITY};
       uint32_t s[MINE];
-#pragma unroll
-      for (int h = 0; h < MINE / 32; ++h) tmem_ld_32x32(s_tmem + 32u * h, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * h));
+      tmem_ld_32x32(s_tmem, s);
       tmem_ld_wait();
-      const int see = lim - KEYS * j - MINE * half;
-      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < MINE; ++i) {
-        const float y = i < see ? __uint_as_float(s[i]) * a.scale_log2 : -INFINITY;
-        s[i] = __float_as_uint(y);
-        top = fmaxf(top, y);
+      for (int i = 0; i < MINE; i += 2) {
+        const f2 y = fma_f2(pack_f2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, none);
+        s[i] = uint32_t(y);
+        s[i + 1] = uint32_t(y >> 32);
       }
-      *to = top;
-      tc_fence_before_sync();
-      ok = all_of(1 + (warp & 3), 64, ok);
+      if (masked)
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) s[i] = i < see ? s[i] : 0xff800000u;
+#pragma unroll
+      for (int i = 0; i < MINE; i += 2) t[(i >> 1) & 1] = max3(t[(i >> 1) & 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+      *to = fmaxf(t[0], t[1]);
+      ok = all_of(1 + (warp & 3), 128, ok);
       if (!ok) break;
-      if (lane == 0) mbar_arrive(s_read);
-      const float mn = fmaxf(m, fmaxf(top, *from)), off = mn == -INFINITY ? 0.0f : mn;
-      const float alpha = ex2(m - off);   // 0 for the first tile
+      const float top = fmaxf(max3(all[0], all[128], all[256]), all[384]);
+      const float mn = fmaxf(m, top), off = mn == -INFINITY ? 0.0f : mn;
+      alpha = ex2(m - off);   // 0 for the first tile
       m = mn;
-      float sum = 0.0f;
-      uint32_t w[3][MINE / 2];
+      const f2 off2 = pack_f2(-off, -off), minus = pack_f2(-1.0f, -1.0f);
+      f2 sum[2] = {0, 0};
 #pragma unroll
-      for (int i = 0; i < MINE / 2; ++i) {
-        const float e0 = ex2(__uint_as_float(s[2 * i]) - off), e1 = ex2(__uint_as_float(s[2 * i + 1]) - off);
-        sum += e0 + e1;
-        w[0][i] = pack2<true>(e0, e1);
-        const float f0 = e0 - __uint_as_float(w[0][i] << 16), f1 = e1 - __uint_as_float(w[0][i] & 0xffff0000u);
-        w[1][i] = pack2<true>(f0, f1);
-        w[2][i] = pack2<true>(f0 - __uint_as_float(w[1][i] << 16), f1 - __uint_as_float(w[1][i] & 0xffff0000u));
+      for (int h = 0; h < 4; ++h) {   // 8 keys
+        if ((h >> 1) >= chunks) break;
+        uint32_t w[3][4];
+        if (8 * h >= most) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[0][i] = w[1][i] = w[2][i] = 0u;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f2 y = add_f2(pack_f2(__uint_as_float(s[8 * h + 2 * i]), __uint_as_float(s[8 * h + 2 * i + 1])), off2);
+            const f2 e = pack_f2(ex2(lo_f2(y)), ex2(hi_f2(y)));
+            sum[i & 1] = add_f2(sum[i & 1], e);
+            auto plane = [&](f2 x) { return pack2<true>(lo_f2(x), hi_f2(x)); };
+            auto less = [&](f2 x, uint32_t p2) { return fma_f2(pack_f2(__uint_as_float(p2 << 16), __uint_as_float(p2 & 0xffff0000u)), minus, x); };   // exact
+            w[0][i] = plane(e);
+            const f2 f = less(e, w[0][i]);
+            w[1][i] = plane(f);
+            w[2][i] = plane(less(f, w[1][i]));
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) tmem_st_32x4(tmem + lanes + place_of_p(2 * part + (h >> 1), q) + 4u * (h & 1), w[q]);
       }
-      if (j > 0) {   // the tile before: when it is done, its sum is taken and its P may be overwritten
-        ok = __all_sync(0xffffffffu, wait_bar(t_bar, (j - 1) & 1, abort_flag, a.status, 79)) && ok;
-        tc_fence_after_sync();
-        add_tile(alpha);
-      }
-#pragma unroll
-      for (int q = 0; q < 3; ++q)
-#pragma unroll
-        for (int h = 0; h < MINE / 32; ++h)
-          tmem_st_32x16(tmem + lanes + Sh::P + uint32_t(KEYS / 2) * q + uint32_t(MINE / 2) * half + 16u * h, *reinterpret_cast<uint32_t(*)[16]>(w[q] + 16 * h));
-      l = fmaf(l, alpha, sum);
+      sum[0] = add_f2(sum[0], sum[1]);
+      l = fmaf(l, alpha, lo_f2(sum[0]) + hi_f2(sum[0]));
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
@@ -335,26 +373,26 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
     if (ok && n > 0) {
       ok = __all_sync(0xffffffffu, wait_bar(t_bar, (n - 1) & 1, abort_flag, a.status, 80));
       tc_fence_after_sync();
-      add_tile(1.0f);
+      add_tile();
     }
     *to = l;
-    ok = all_of(1 + (warp & 3), 64, ok);
+    ok = all_of(1 + (warp & 3), 128, ok);
     if (ok && mine) {
-      l += *from;
-      float* out = static_cast<float*>(a.out) + int64_t(q0 + token) * a.out_stride + int64_t(head) * a.D + (D / 2) * half;
-      const int cols = a.D - (D / 2) * half;
+      l = (all[0] + all[128]) + (all[256] + all[384]);
+      float* out = static_cast<float*>(a.out) + int64_t(q0 + token) * a.out_stride + int64_t(head) * a.D + (D / 4) * part;
+      const int cols = a.D - (D / 4) * part;
       if (any)
 #pragma unroll 1
         for (int key = 0; key < lim; ++key) {
           if (!p.odd_v[int64_t(k0 + key) * a.G + g]) continue;
-          const float* v = static_cast<const float*>(a.v) + int64_t(k0 + key) * a.kv_stride + int64_t(g) * a.D + (D / 2) * half;
+          const float* v = static_cast<const float*>(a.v) + int64_t(k0 + key) * a.kv_stride + int64_t(g) * a.D + (D / 4) * part;
 #pragma unroll
-          for (int i = 0; i < D / 2; ++i)
+          for (int i = 0; i < D / 4; ++i)
             if (i < cols && !(fabsf(v[i]) <= 3.402823466e38f)) o[i] += v[i];
         }
       const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
-      for (int i = 0; i < D / 2; i += 4) {
+      for (int i = 0; i < D / 4; i += 4) {
         float r[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[e] = l == 0.0f ? 0.0f : o[i + e] / l;
@@ -382,8 +420,8 @@ static int f3_launch(F3Args p, const uint8_t* q, const uint8_t* k, const uint8_t
   p.tpt = 128 / a.rep;
   p.q = reinterpret_cast<const uint16_t*>(q);
   CUtensorMap mk, mv;
-  if (int rc = attn_tensor_map(&mk, true, k, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, F3Shape<D>::KEYS)) return rc;
-  if (int rc = attn_tensor_map(&mv, true, v, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, F3Shape<D>::KEYS)) return rc;
+  if (int rc = attn_tensor_map(&mk, true, k, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, 64)) return rc;
+  if (int rc = attn_tensor_map(&mv, true, v, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, 64)) return rc;
   auto kern = attn_prompt_f32_tc_kernel<D>;
   SIMP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(F3Shape<D>::SMEM)));
   const int64_t units = std::min(a.total_q, a.total_q / p.tpt + a.n_seqs) * a.G;

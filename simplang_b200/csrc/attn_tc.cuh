@@ -35,6 +35,9 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t t, uint32_t (&r)[16]) {
       : "r"(t)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_32x4(uint32_t t, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0, %1, %2, %3};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(t) : "memory");
+}
 __device__ __forceinline__ void tmem_st_32x8(uint32_t t, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
                "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(t)
