@@ -1,8 +1,8 @@
-"""Per-op sweep of the bandwidth-bound kernels (f32 GEMV, W4 GEMV, rmsnorm, softmax, silu) and of the
-int8 GEMM at the configured shapes.  Prints one JSON line per case with the achieved GB/s (or TOPS), the
+"""Per-op sweep of the bandwidth-bound kernels (f32 GEMV, W4 GEMV, rmsnorm, softmax, silu), of the
+int8 GEMM and of the batched serving ops (prompt attention, the 8-bit cache, logits) at the configured shapes.  Prints one JSON line per case with the achieved GB/s (or TOPS), the
 algorithmic bytes used, and the fraction of the measured roofline.
 
-    python -m simplang_b200.opbench [--iters 50] [--only gemv_f32,gemm_f32,w4,rowops,gemm_i8,gemm_i4,mma_peak,decode110m,decode3b,decode_i8,prefill_i8]
+    python -m simplang_b200.opbench [--iters 50] [--only gemv_f32,gemm_f32,w4,rowops,gemm_i8,gemm_i4,mma_peak,prompt,kv8,logits,decode110m,decode3b,decode_i8,prefill_i8]
 
 Each case rotates over enough independent operand copies that the working set exceeds twice the
 126 MB L2, so every iteration streams from HBM the way consecutive layers of a decode step do.
@@ -364,6 +364,93 @@ def bench_prefill_i8():
     m.close()
 
 
+# (query heads, key/value heads, head size) of the configured models
+SERVING_HEADS = {"110m": (12, 12, 64), "3b": (32, 32, 100), "1b": (32, 8, 64)}
+
+
+def serving_rows(rng, rows, width, dtype):
+    """Random rows as the 16- or 32-bit words of `dtype`."""
+    x = rng.standard_normal((rows, width), dtype=np.float32)
+    if dtype == sg.F16:
+        return sg.DeviceBuffer.from_numpy(x.astype(np.float16))
+    return sg.DeviceBuffer.from_numpy((x.view(np.uint32) >> 16).astype(np.uint16) if dtype == sg.BF16 else x)
+
+
+def i32(values):
+    return sg.DeviceBuffer.from_numpy(np.asarray(values, np.int32))
+
+
+def bench_prompt(iters):
+    """Causal attention over packed prompts; the rate counts 4 * head size operations per pair of a query and a key that
+    it sees.  No copies: operands of a few MB that every block reads again are in L2 in a model's step too."""
+    rng = np.random.default_rng(6)
+    for model, dtype, name, n, length in [("110m", sg.F32, "f32", 1, 1024), ("110m", sg.F32, "f32", 8, 512), ("3b", sg.F32, "f32", 1, 2048),
+                                          ("1b", sg.BF16, "bf16", 32, 128), ("1b", sg.BF16, "bf16", 8, 1024), ("1b", sg.F16, "f16", 1, 8192),
+                                          ("3b", sg.F16, "f16", 4, 2048)]:
+        H, G, D = SERVING_HEADS[model]
+        if not want((n, length, H, G, D)):
+            continue
+        rows, size = n * length, 4 if dtype == sg.F32 else 2
+        q, k, v = (serving_rows(rng, rows, heads * D, dtype) for heads in (H, G, G))
+        out = sg.DeviceBuffer(rows * H * D * size)
+        off = i32(np.arange(n + 1) * length)
+        ms = timed(lambda i: sg.attn_prompt(q, k, v, out, off, off, n, rows, rows, H, G, D, dtype=dtype), 1, iters)
+        flop = 4.0 * D * H * n * (length * (length + 1) // 2)
+        emit("attn_prompt_" + name, [n, length, H, G, D], ms, rows * (2 * H + 2 * G) * D * size, {"tflops": round(flop / (ms * 1e-3) / 1e12, 1)})
+
+
+def bench_kv8(iters):
+    """The 8-bit cache: attention of one token per sequence (bytes of the cache), and rows written and read."""
+    rng = np.random.default_rng(7)
+    bt = 64
+    for model, dtype, name, n, length in [("110m", sg.F32, "f32", 1, 1024), ("3b", sg.F32, "f32", 16, 2048), ("1b", sg.BF16, "bf16", 1, 65536),
+                                          ("1b", sg.BF16, "bf16", 64, 4096)]:
+        H, G, D = SERVING_HEADS[model]
+        if not want((n, length, H, G, D)):
+            continue
+        per, size = (length + bt - 1) // bt, 4 if dtype == sg.F32 else 2
+        blocks, rows = n * per, n * length
+        kb, vb, ksb, vsb = sg.kv8_bytes(blocks, bt, G, D)
+        nc = max(1, min(8, copies_for(kb + vb)))
+        caches = [[sg.DeviceBuffer(b) for b in (kb, vb, ksb, vsb)] for _ in range(nc)]
+        handles = [sg.kv8_cache(*c, blocks, bt, G, D) for c in caches]
+        table = i32(rng.permutation(blocks).reshape(n, per))
+        k, v = (serving_rows(rng, rows, G * D, dtype) for _ in range(2))
+        off, starts, lengths = i32(np.arange(n + 1) * length), i32(np.zeros(n)), i32(np.full(n, length))
+        moved = 2 * rows * G * D * (size + 1)
+        ms = timed(lambda i: sg.kv8_append(handles[i], table, per, k, v, off, starts, n, rows, dtype=dtype), nc, iters)
+        emit("kv8_append_" + name, [n, length, H, G, D], ms, moved, {"copies": nc})
+        for h in handles:
+            sg.kv8_append(h, table, per, k, v, off, starts, n, rows, dtype=dtype)
+        ms = timed(lambda i: sg.kv8_read(handles[i], table, per, k, v, off, starts, n, rows, dtype=dtype), nc, iters)
+        emit("kv8_read_" + name, [n, length, H, G, D], ms, moved, {"copies": nc})
+        q, out = serving_rows(rng, n, H * D, dtype), sg.DeviceBuffer(n * H * D * size)
+        ms = timed(lambda i: sg.attn_kv8(handles[i], table, per, q, out, lengths, n, length, H, dtype=dtype), nc, iters)
+        emit("attn_kv8_" + name, [n, length, H, G, D], ms, kb + vb + ksb + vsb + 2 * n * H * D * size, {"copies": nc})
+        del caches, handles
+
+
+def bench_logits(iters):
+    """Penalties of a history of 1024 tokens, 16 biases, a mask and the greedy choice."""
+    rng = np.random.default_rng(8)
+    for rows, vocab in [(1, 32000), (32, 32000), (1, 128256), (128, 128256)]:
+        if not want((rows, vocab)):
+            continue
+        words = (vocab + 31) // 32
+        nb = rows * (8 * vocab + 4 * words + 4 * 1024)
+        nc = min(8, copies_for(nb))
+        x = [sg.DeviceBuffer.from_numpy(rng.standard_normal((rows, vocab), dtype=np.float32)) for _ in range(nc)]
+        y, best = [sg.DeviceBuffer(4 * rows * vocab) for _ in range(nc)], sg.DeviceBuffer(4 * rows)
+        per_row = sg.DeviceBuffer.from_numpy(np.full(rows, 1.25, np.float32))
+        keep = [i32(rng.integers(0, vocab, rows * 1024)), i32(np.arange(rows + 1) * 1024), i32(rng.integers(0, vocab, rows * 16)),
+                sg.DeviceBuffer.from_numpy(rng.standard_normal(rows * 16).astype(np.float32)), i32(np.arange(rows + 1) * 16),
+                sg.DeviceBuffer.from_numpy(rng.integers(0, 1 << 32, (rows, words), dtype=np.uint32))]
+        rules = sg.logits_rules(keep[0], keep[1], rows * 1024, per_row, per_row, per_row, keep[2], keep[3], keep[4], rows * 16, keep[5], words)
+        ms = timed(lambda i: sg.logits_process(x[i], y[i], rows, vocab, rules, argmax=best), nc, iters)
+        emit("logits_process_f32", [rows, vocab], ms, nb, {"copies": nc})
+        del x, y
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--iters", type=int, default=50)
@@ -398,6 +485,12 @@ def main():
         bench_gemm_i4(args.iters)
     if "mma_peak" in which:
         bench_mma_peak(args.iters)
+    if "prompt" in which:
+        bench_prompt(args.iters)
+    if "kv8" in which:
+        bench_kv8(args.iters)
+    if "logits" in which:
+        bench_logits(args.iters)
     if "decode110m" in which:
         bench_decode("110m")
     if "decode3b_marks" in which:
