@@ -1,10 +1,13 @@
 // attn_prompt.cu -- causal attention over prompts: packed sequences of different lengths, grouped heads.
 //
-// This file holds the entry point and the f32 kernel, which serves every type, head size and alignment; 16-bit types with
-// head sizes 64 and 128 run on the tensor cores (attn_prompt_tc.cu).
+// This file holds the entry point and the FFMA kernel.  Heads of up to 128 elements run on the tensor cores: f16 and bf16 in
+// attn_prompt_tc.cu, f32 in attn_prompt_f32_tc.cu.  The FFMA kernel does what those cannot: scale <= 0 for 16-bit types,
+// calls without keys or with more rows than their tensor maps address, and calls for which no scratch can be had (inside a
+// recording that would have to grow it).
 //
-// f32 kernel: one block per 64 queries of one head.  Scores of 64 keys at a time, the running maximum and sum of the
-// softmax per row, one pass over K and V.  Bound by FFMA and the shared-memory loads that feed it.
+// FFMA kernel: one block per 64 queries of one head.  Scores of 64 keys at a time, the running maximum and sum of the softmax
+// per row, one pass over K and V.  Bound by FFMA and the shared-memory loads that feed it: 32 heads of 100, 2048 f32 tokens
+// 1010 us, where the tensor cores take 260.
 #include <algorithm>
 #include <climits>
 

@@ -10,7 +10,11 @@
 //   warps 4-11, 12-19  softmax of tile A, of tile B: two threads per row, 64 keys each, which exchange their maxima
 // P (16 bits) overwrites S in place: S_X(j + 1) is issued behind O_X += P_X(j) V(j) by the same thread, whose MMAs run in order.
 // While the tensor cores work on one tile, the other tile's softmax runs: 2 x 128 x 128 x D MACs take 4 D cycles per tile and
-// step, its 16384 exponentials 1024, so for D = 128 both are busy about half of the time.
+// step, its 16384 exponentials 1024.  Measured for D = 128 (one prompt of 8192, 32 / 8 heads: 543 us, 1012 TFLOP/s, 0.62 of
+// the measured rate): both tiles' steps take 3800 cycles, a tile's chain of 1700 softmax, 200 maxima, 100 P, 250 hand-over,
+// 1250 MMAs and 250 hand-over back.  The tensor cores and the exponentials are each busy a little over half of the time; the
+// softmax is held up by its two warps per scheduler issuing in order (exponentials in polynomial form on the FMA pipe cost
+// more issue slots than they save: an eighth of them 564 us, a quarter 577).
 //
 // Softmax: the row's running maximum moves only when a tile exceeds it by more than 2^8 (weights are then at most 2^8, well
 // inside f16), so O is rarely rescaled: it stays in TMEM.  S_X(j + 1) being complete implies that P_X(j) V(j) is, so the
@@ -382,29 +386,41 @@ __global__ void __launch_bounds__(128 + 256 * TILES, 3 - TILES)
         float t[2] = {-INFINITY, -INFINITY};
         f2 sum[2] = {0, 0};
         uint32_t s[2][16], w[32];   // 16 scores at a time, the next 16 on their way: room for exponentials in flight
-        tmem_ld_32x16(s_tmem + 64u * half, s[0]);
+        // Tiles that every row sees have a form without branches where heads of 64 leave the softmax alone on the critical path
+        // (8192 tokens, 32 / 8 heads: 497 -> 465 us).  Heads of 128: 543 -> 526 us there, but 113 -> 118 for 16 prompts of 512
+        // and 146 -> 149 for 8 of 1024, whose blocks go through the code of both forms for few tiles each.
+        auto weigh = [&](auto all_seen) {
+          constexpr bool ALL = decltype(all_seen)::value;
+          tmem_ld_32x16(s_tmem + 64u * half, s[0]);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          uint32_t(&v)[16] = s[h & 1];
-          tmem_ld_wait();
-          if (16 * h >= most) {
+          for (int h = 0; h < 4; ++h) {
+            uint32_t(&v)[16] = s[h & 1];
+            tmem_ld_wait();
+            if (!ALL && 16 * h >= most) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[8 * h + i] = 0u;
-            continue;
+              for (int i = 0; i < 8; ++i) w[8 * h + i] = 0u;
+              continue;
+            }
+            if (h < 3) tmem_ld_32x16(s_tmem + 64u * half + 16u * (h + 1), s[(h + 1) & 1]);
+            if (!ALL && masked) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = 16 * h + i < see ? v[i] : 0xff800000u;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              t[i & 1] = max3(t[i & 1], __uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+              const f2 y = fma_f2(pack_f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, off2);
+              const f2 e = pack_f2(ex2(lo_f2(y)), ex2(hi_f2(y)));
+              sum[i & 1] = add_f2(sum[i & 1], e);
+              w[8 * h + i] = pack2<BF16>(lo_f2(e), hi_f2(e));
+            }
           }
-          if (h < 3) tmem_ld_32x16(s_tmem + 64u * half + 16u * (h + 1), s[(h + 1) & 1]);
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = 16 * h + i < see ? v[i] : 0xff800000u;
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            t[i & 1] = max3(t[i & 1], __uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-            const f2 y = fma_f2(pack_f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, off2);
-            const f2 e = pack_f2(ex2(lo_f2(y)), ex2(hi_f2(y)));
-            sum[i & 1] = add_f2(sum[i & 1], e);
-            w[8 * h + i] = pack2<BF16>(lo_f2(e), hi_f2(e));
-          }
+        };
+        if constexpr (D == 64 && TILES == 2) {
+          if (masked) weigh(std::false_type());
+          else weigh(std::true_type());
+        } else {
+          weigh(std::false_type());
         }
         float top = fmaxf(t[0], t[1]);
         if (attempt == 0) *to = top;
