@@ -37,7 +37,7 @@ __device__ __forceinline__ unsigned long long logit_key(float v, int i) {
 // A thread has U 16-byte vectors in flight; a block works on NSUB times LG_THREADS * U * VEC tokens.
 template <typename T, int U, int NSUB>
 __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) {
-  constexpr int VEC = 16 / sizeof(T), SUB = LG_THREADS * U * VEC, SLICE = SUB * NSUB;
+  constexpr int VEC = 16 / sizeof(T), SUB = LG_THREADS * U * VEC, SLICE = SUB * NSUB, LISTED = SLICE / 8;
   extern __shared__ __align__(16) int lg_smem[];
   __shared__ unsigned long long wbest[LG_THREADS / 32];
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
@@ -77,6 +77,8 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
   int* changed = lg_smem;                                             // [SLICE]
   uint32_t* bits = reinterpret_cast<uint32_t*>(lg_smem + SLICE);      // [SLICE / 32]
   uint32_t* biased = bits + SLICE / 32;                               // [SLICE / 32]
+  int* n_listed = lg_smem + SLICE + SLICE / 16;                       // the history's tokens in this slice, each once, so that
+  uint16_t* listed = reinterpret_cast<uint16_t*>(n_listed + 4);       // warps work on whole lots of them: [LISTED]
   const bool sparse = a.r.tokens || a.r.bias_tokens;
   if (sparse) {
     int hb = 0, he = 0, bb = 0, be = 0;
@@ -92,6 +94,7 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
         ids[k] = id >= first && id < last ? id - base : -1;
       }
     };
+    if (tid == 0) *n_listed = 0;
     fetch(hb);
     const int bias0 = a.r.bias_tokens && bb + tid < be ? __ldg(a.r.bias_tokens + bb + tid) : -1;
     for (int i = 4 * tid; i < SLICE + SLICE / 16; i += 4 * LG_THREADS) *reinterpret_cast<int4*>(lg_smem + i) = make_int4(0, 0, 0, 0);
@@ -118,34 +121,34 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
       for (int i0 = hb;;) {
 #pragma unroll
         for (int k = 0; k < E; ++k)
-          if (ids[k] >= 0) atomicAdd(changed + ids[k], 1);
+          if (ids[k] >= 0 && atomicAdd(changed + ids[k], 1) == 0)
+            if (const int at = atomicAdd(n_listed, 1); at < LISTED) listed[at] = uint16_t(ids[k]);
         i0 += E * LG_THREADS;
         if (i0 >= he) break;
         fetch(i0);
       }
     }
     twice = __syncthreads_or(twice);
-    if (he > hb) {
-      for (int i0 = hb;;) {
-        if (he - hb > E * LG_THREADS) fetch(i0);
-        float v[E];
-#pragma unroll
-        for (int k = 0; k < E; ++k) {   // the first of a token's places works for all
-          if (ids[k] < 0) continue;
-          const uint32_t bit = 1u << (ids[k] & 31);
-          if (atomicOr(bits + (ids[k] >> 5), bit) & bit) ids[k] = -1;
-        }
-#pragma unroll
-        for (int k = 0; k < E; ++k) v[k] = ids[k] >= 0 ? to_f32(in[base + ids[k]]) : 0.0f;
-#pragma unroll
-        for (int k = 0; k < E; ++k) {
-          if (ids[k] < 0) continue;
-          // separate roundings, so that the result does not hang on a contraction
-          const float f = v[k] > 0.0f ? __fdiv_rn(v[k], rep) : __fmul_rn(v[k], rep);
-          changed[ids[k]] = __float_as_int(__fsub_rn(f, __fadd_rn(__fmul_rn(freq, float(changed[ids[k]])), pres)));
-        }
-        i0 += E * LG_THREADS;
-        if (i0 >= he) break;
+    auto penalise = [&](int id) {
+      const float v = to_f32(in[base + id]);
+      // separate roundings, so that the result does not hang on a contraction
+      const float f = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+      changed[id] = __float_as_int(__fsub_rn(f, __fadd_rn(__fmul_rn(freq, float(changed[id])), pres)));
+    };
+    if (const int n = *n_listed; n > LISTED) {   // too many to list: the first of a token's places in the history works for all
+      for (int i = hb + tid; i < he; i += LG_THREADS) {
+        int id = __ldg(a.r.tokens + i);
+        if (id < first || id >= last) continue;
+        id -= base;
+        const uint32_t bit = 1u << (id & 31);
+        if (!(atomicOr(bits + (id >> 5), bit) & bit)) penalise(id);
+      }
+      __syncthreads();
+    } else if (n > 0) {
+      for (int i = tid; i < n; i += LG_THREADS) {
+        const int id = listed[i];
+        atomicOr(bits + (id >> 5), 1u << (id & 31));
+        penalise(id);
       }
       __syncthreads();
     }
@@ -256,7 +259,7 @@ static int logits_run(LogitsArgs& a) {
     a.key = reinterpret_cast<unsigned long long*>(p);
     a.arrived = reinterpret_cast<int*>(p + size_t(65536) * 8);
   }
-  const size_t smem = a.r.tokens || a.r.bias_tokens ? size_t(SLICE) * 4 + SLICE / 4 : 0;
+  const size_t smem = a.r.tokens || a.r.bias_tokens ? size_t(SLICE) * 4 + SLICE / 4 + 16 + SLICE / 4 : 0;
   auto kern = logits_kernel<T, U, NSUB>;
   if (smem > 32 * 1024) SIMP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
   SIMP_CUDA(launch_kernel(kern, grid, dim3(LG_THREADS), smem, ctx().stream, true, a));
@@ -264,7 +267,7 @@ static int logits_run(LogitsArgs& a) {
 }
 
 // Slices of 8192 tokens where that still gives every SM two blocks, else of 1024 (f32) or 2048.  200 rows of 128256 with
-// histories of 2000: 57 us with 8192, 64 with 16384 (three blocks per SM), 76 with 4096 (histories read twice as often);
+// histories of 2000: 55 us with 8192, 62 with 16384 (three blocks per SM), 66 with 4096 (histories read twice as often);
 // without history and biases 36 us, 0.87 of the memory's rate.
 template <typename T>
 static int logits_launch(LogitsArgs& a) {

@@ -217,3 +217,15 @@ def test_long_lists(gpu, rows, vocab, biases):
     want = torch.from_numpy(expected(c))
     out, best = run(gpu, c)
     assert equal(out, want) and np.array_equal(best, greedy(want))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,history,biases", [(300, 8193, 4000, 40), (150, 16400, 300, 600), (2, 3000, 9000, 4)])
+def test_rows_of_long_histories(gpu, dtype, rows, vocab, history, biases):
+    """Histories with more different tokens in a block's slice than it lists, and rows with fewer, in long and short slices."""
+    c = make(rows + vocab, rows, vocab, dtype, history, biases, "one")
+    want = torch.from_numpy(expected(c)).to(TYPES[dtype])
+    for inplace in (False, True):
+        out, best = run(gpu, c, inplace)
+        assert equal(out, want), f"{(out != want).sum()} logits differ"
+        assert np.array_equal(best, greedy(want))
