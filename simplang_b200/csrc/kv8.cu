@@ -384,7 +384,7 @@ template <int S, int PLANES, int NH>
 __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Args a) {
   constexpr int P = 32 * S, HEADS = 4 * NH, NT = NH + (PLANES == 3 ? 1 : 0), STEP = 32 * AK_WARPS;
   constexpr int STAGES = AttnKv8Ring<S>::STAGES, STAGE = AttnKv8Ring<S>::STAGE;
-  constexpr float QMAX = PLANES == 3 ? 8323072.0f : 32512.0f;      // 127 << 16, 127 << 8: top byte never overflows
+  constexpr float QMAX = float(127 << (8 * (PLANES - 1)));          // the top byte never overflows
   constexpr float PMAX = PLANES == 3 ? 16777215.0f : 65535.0f;
   extern __shared__ __align__(128) uint8_t ak_ring[];              // [warp][stage][K 32 x P, V 2 x P x 16]; at the end [warp][head][P] sums
   __shared__ __align__(16) int8_t qb[NT * 8][P];                   // byte planes, one row per B column

@@ -212,7 +212,7 @@ def attention_tolerance(c64, table, lengths, q, scale, dtype, ref):
     2^-20 of exponentials; as integers they are off by half of 1 / 65535 (f32: 2^-24) of the largest of their 32, which is at
     most 32 / 65535 / 2 of the whole; sums of n / 32 tile results are f32.  One output rounding."""
     t = TYPES[dtype]
-    step, weight = (0.5 / 8323072, 32 * 0.5 / 16777215) if dtype == "f32" else (0.5 / 32512, 32 * 0.5 / 65535)
+    step, weight = (0.5 / (127 << 16), 32 * 0.5 / 16777215) if dtype == "f32" else (0.5 / 32512, 32 * 0.5 / 65535)
     tol = 0.0
     for s, n in enumerate(lengths):
         if not n:
