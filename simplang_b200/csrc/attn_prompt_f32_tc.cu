@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
           mbar_arrive_expect_tx(k_full(s), boxes(j) * (Sh::PLANE / 2));
           plane(&map_k, k_smem, k_full(s), s, j);
         }
-        ok = j == 0 || wait_bar(t_bar, (j - 1) & 1, abort_flag, a.status, 81);
+        ok = j == 0 || wait_bar(t_bar, (j - 1) & 1, abort_flag, a.status, 82);
         if (!ok) break;
         mbar_arrive_expect_tx(v_full, boxes(j) * (Sh::STAGE / 2));
         for (int s = 0; s < 3; ++s) plane(&map_v, v_smem, v_full, s, j);
