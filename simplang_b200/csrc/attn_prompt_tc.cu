@@ -608,21 +608,40 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(const AttnPack q, const 
   uint4 out[3];
   uint16_t* h = reinterpret_cast<uint16_t*>(out);
   bool bad = false;
+  if constexpr (SPLIT) {
+    uint32_t most = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if constexpr (SPLIT) {
-      float x = e8[e];
-      if (!(fabsf(x) <= 3.402823466e38f)) bad = true, x = 0.0f;
-      uint16_t a = __bfloat16_as_ushort(__float2bfloat16_rn(x));
-      if ((a & 0x7fffu) == 0x7f80u) --a;   // the largest f32 would round to infinity
-      const float r = x - __uint_as_float(uint32_t(a) << 16);
-      const __nv_bfloat16 b = __float2bfloat16_rn(r);
-      h[e] = a;
-      h[8 + e] = __bfloat16_as_ushort(b);
-      h[16 + e] = __bfloat16_as_ushort(__float2bfloat16_rn(r - __bfloat162float(b)));
+    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(e8[e]) & 0x7fffffffu);
+    if (most < 0x7f7f8000u) {   // everything is finite and rounds to a finite bf16
+      uint32_t* w = reinterpret_cast<uint32_t*>(out);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f2 minus = pack_f2(-1.0f, -1.0f);
+        f2 x = pack_f2(e8[2 * e], e8[2 * e + 1]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          const uint32_t p = pack2<true>(lo_f2(x), hi_f2(x));
+          w[4 * q + e] = p;
+          if (q < 2) x = fma_f2(pack_f2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u)), minus, x);   // exact
+        }
+      }
     } else {
-      h[e] = e8[e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float x = e8[e];
+        if (!(fabsf(x) <= 3.402823466e38f)) bad = true, x = 0.0f;
+        uint16_t a = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+        if ((a & 0x7fffu) == 0x7f80u) --a;   // the largest f32 would round to infinity
+        const float r = x - __uint_as_float(uint32_t(a) << 16);
+        const __nv_bfloat16 b = __float2bfloat16_rn(r);
+        h[e] = a;
+        h[8 + e] = __bfloat16_as_ushort(b);
+        h[16 + e] = __bfloat16_as_ushort(__float2bfloat16_rn(r - __bfloat162float(b)));
+      }
     }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = e8[e];
   }
   if (in) {
     const int64_t plane = rows * per;
