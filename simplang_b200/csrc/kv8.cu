@@ -347,6 +347,7 @@ struct AttnKv8Args {
   int* status;
   float scale_log2;   // scale * log2(e)
   int rep, max_len, chunk, max_chunks, dtype;
+  bool cluster;       // the chunks of a (sequence, head group) are one thread-block cluster
 };
 
 constexpr int AK_WARPS = 4, AK_JOIN = 8;
@@ -390,6 +391,7 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
   __shared__ __align__(16) int8_t qb[NT * 8][P];                   // byte planes, one row per B column
   __shared__ float qs[HEADS];
   __shared__ float om[AK_WARPS][HEADS], ol[AK_WARPS][HEADS];
+  __shared__ __align__(8) float2 joined[HEADS];                    // this block's top and sum of each head
   __shared__ __align__(8) uint64_t bars[AK_WARPS][STAGES];
   __shared__ int last, abort_flag;
   const Kv8View& c = a.c;
@@ -419,6 +421,10 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
   if (chunk >= n_chunks) {
     if (len == 0 && chunk == 0)
       for (int i = threadIdx.x; i < nh * c.D; i += blockDim.x) store_any(a.out, orow + i, 0.0f, a.dtype);
+    if (a.cluster && n_chunks > 1) {   // the others' barriers
+      ptx::cluster_sync_all();
+      ptx::cluster_sync_all();
+    }
     return;
   }
   const int c1 = min(len, c0 + a.chunk);
@@ -708,6 +714,9 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
     }
     if (n_chunks == 1) {
       finish(h, d, val, den);
+    } else if (a.cluster) {
+      reinterpret_cast<float*>(ak_ring)[i] = val;   // (read by this thread only, above)
+      if (d == 0) joined[h] = make_float2(top, den);
     } else {
       part[2 * HEADS + i] = val;
       if (d == 0) {
@@ -717,15 +726,8 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
     }
   }
   if (n_chunks == 1) return;
-  // ---- the last chunk of this (sequence, head group) to arrive joins all of them, in their order
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(a.count + slot, 1) == n_chunks - 1;
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  const float* all = a.part + slot * a.max_chunks * PART;
-  for (int i = 4 * threadIdx.x; i < nh * P; i += 4 * blockDim.x) {
+  // ---- all chunks of this (sequence, head group), in their order, element i .. i + 3; part(x) is chunk x's
+  auto join = [&](int i, auto part) {
     const int h = i / P, d = i - h * P;
     float top = -INFINITY, den = 0.0f;
     float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -734,9 +736,7 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
       float4 v[AK_JOIN];
 #pragma unroll
       for (int x = 0; x < AK_JOIN; ++x) {
-        const float* p = all + int64_t(min(x0 + x, n_chunks - 1)) * PART;
-        md[x] = __ldcg(reinterpret_cast<const float2*>(p + 2 * h));
-        v[x] = __ldcg(reinterpret_cast<const float4*>(p + 2 * HEADS + i));
+        part(min(x0 + x, n_chunks - 1), h, i, md[x], v[x]);
         if (x0 + x >= n_chunks) md[x].x = -INFINITY;
       }
       float now = top;
@@ -757,7 +757,35 @@ __global__ void __launch_bounds__(AK_WARPS * 32) attn_kv8_kernel(const AttnKv8Ar
     finish(h, d + 1, val.y, den);
     finish(h, d + 2, val.z, den);
     finish(h, d + 3, val.w, den);
+  };
+  if (a.cluster) {   // out of the blocks' shared memory, every block its share of the elements
+    __syncwarp();
+    ptx::cluster_sync_all();
+    const uint32_t sums = ptx::smem_u32(ak_ring), heads = ptx::smem_u32(joined);
+    for (int i = 4 * (threadIdx.x * n_chunks + chunk); i < nh * P; i += 4 * blockDim.x * n_chunks)
+      join(i, [&](int x, int h, int at, float2& md, float4& v) {
+        const uint32_t m2 = ptx::cluster_map(heads + 8 * h, x), v4 = ptx::cluster_map(sums + 4 * at, x);
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(md.x), "=f"(md.y) : "r"(m2));
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(v4));
+      });
+    __syncwarp();
+    ptx::cluster_sync_all();   // nobody leaves while another reads its memory
+    return;
   }
+  // out of global memory, by the chunk that arrives last
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(a.count + slot, 1) == n_chunks - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  const float* all = a.part + slot * a.max_chunks * PART;
+  for (int i = 4 * threadIdx.x; i < nh * P; i += 4 * blockDim.x)
+    join(i, [&](int x, int h, int at, float2& md, float4& v) {
+      const float* p = all + int64_t(x) * PART;
+      md = __ldcg(reinterpret_cast<const float2*>(p + 2 * h));
+      v = __ldcg(reinterpret_cast<const float4*>(p + 2 * HEADS + at));
+    });
   if (threadIdx.x == 0) a.count[slot] = 0;
 }
 
@@ -766,7 +794,22 @@ static cudaError_t attn_kv8_launch(int nh, dim3 grid, cudaStream_t st, const Att
   auto kern = nh == 1 ? attn_kv8_kernel<S, PLANES, 1> : attn_kv8_kernel<S, PLANES, 2>;
   constexpr size_t smem = AttnKv8Ring<S>::SMEM;
   if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)); e != cudaSuccess) return e;
-  return launch_kernel(kern, grid, dim3(AK_WARPS * 32), smem, st, true, a);
+  if (!a.cluster) return launch_kernel(kern, grid, dim3(AK_WARPS * 32), smem, st, true, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(AK_WARPS * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = grid.x;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 // ------------------------------------------------------------------------------------------------ arguments
@@ -879,15 +922,28 @@ SIMP_API int simp_gpu_attn_kv8(const simp_kv8_cache* cache, const int32_t* block
   const int64_t groups = int64_t(a.c.G) * ((a.rep + 4 * nh - 1) / (4 * nh));
   const int64_t slots = n_seqs * groups;
   SIMP_REQUIRE(groups <= 65535, SIMP_ERR_SHAPE, "attn_kv8: too many heads");
-  // Chunks of at least a tile per warp.  One sequence: as many blocks as run at once (three per SM), for joining costs as
-  // much as it gains beyond that (131072 tokens, 8 x 128: 56 us with 54 chunks, 67 with 109, 87 with 205).  Several, whose
-  // lengths differ: twice as many and none longer than 2048 tokens, so that the longest does not end alone (64 sequences of
-  // up to 8097: 126 us, 135 in one chunk each, 131 with 1024).
-  const int64_t least = 32 * AK_WARPS, waves = n_seqs == 1 ? 3 : 6, want = std::max<int64_t>(1, waves * int64_t(ctx().sm_count) / slots);
+  // Chunks of at least a tile per warp.  One sequence: as many blocks as run at once (three per SM; 131072 tokens, 8 x 128: 56 us
+  // with 54 chunks, 67 with 109, 87 with 205).  Several, whose lengths differ: twice as many and none longer than 2048 tokens, so
+  // that the longest does not end alone (64 sequences of up to 8097: 126 us, 135 in one chunk each, 131 with 1024).  But no more
+  // than 32 (64 from 32768 tokens on), for the block that arrives last joins eight at a time: 16384 tokens of 1 x 128 with 8
+  // query heads 19 us with 32, 23 with 64, 35 with 128; 131072 tokens 58, 45 and 93 (with 444).
+  const int64_t least = 32 * AK_WARPS, waves = n_seqs == 1 ? 3 : 6, most = max_len < 32768 ? 32 : 64;
+  const int64_t want = std::min(most, std::max<int64_t>(1, waves * int64_t(ctx().sm_count) / slots));
   a.chunk = int(std::max(least, cdiv(cdiv(std::max<int64_t>(max_len, 1), want), least) * least));
   if (n_seqs > 1) a.chunk = std::min(a.chunk, 2048);
   a.max_chunks = int(std::max<int64_t>(1, cdiv(max_len, a.chunk)));
-  if (a.max_chunks > 1) {
+  // Up to 4096 tokens where all blocks run at once: eight chunks at most, a cluster that joins them out of its shared memory,
+  // which takes 1.3 us where global memory takes 2.8.  1024 tokens, 8 x 64: 6.2 -> 5.4 us, 2048: 7.7 -> 6.8, 4096: 9.8 -> 9.2, but
+  // 8192: 11.1 -> 13.4.  (Clusters that do not all fit at once: 8 sequences of 1024, 8 x 64: 7.3 -> 11.8.)
+  if (a.max_chunks > 1 && max_len <= 4096) {
+    const int64_t share = cdiv(cdiv(max_len, AK_JOIN), least) * least, parts = cdiv(max_len, share);
+    if (slots * parts <= 3 * int64_t(ctx().sm_count)) {
+      a.cluster = true;
+      a.chunk = int(share);
+      a.max_chunks = int(parts);
+    }
+  }
+  if (a.max_chunks > 1 && !a.cluster) {
     a.part = static_cast<float*>(scratch(size_t(slots) * a.max_chunks * 4 * nh * (a.c.pitch + 2) * 4, SCRATCH_KV8_PART));
     if (!a.part) return scratch_failed("attn_kv8");
     a.count = static_cast<int*>(scratch(size_t(slots) * 4, SCRATCH_KV8_COUNT, true));

@@ -296,6 +296,46 @@ def test_long_cache_is_split_and_joined(gpu, dtype, H, G, dim):
     rec2.close()
 
 
+@pytest.mark.parametrize("dtype,H,G,dim", [("f32", 4, 1, 64), ("bf16", 8, 1, 128), ("f16", 6, 2, 100), ("f32", 12, 12, 33)])
+def test_chunks_joined_in_a_cluster(gpu, dtype, H, G, dim):
+    """Up to eight chunks, of which a sequence needs none, one, some or all; the same bits each time, recorded too, for other
+    lengths, and beside a length that is refused."""
+    rng = np.random.default_rng(15)
+    lengths, bt, top = [1500, 129, 0, 128, 700, 1], 16, 1700
+    table, blocks = make_table([top] * len(lengths), bt, rng)
+    c64 = Cache64(blocks, bt, G, dim, rng)
+    for w in range(2):
+        c64.s[w] *= (2.0 ** rng.integers(-4, 3, c64.s[w].shape)).astype(np.float32)
+    dc = DeviceCache(gpu, c64)
+    q = rows(rng, len(lengths), H, dim, dtype)
+    scale = dim ** -0.5
+
+    def right(got, lengths):
+        ref = reference(c64, table, q, lengths, scale)
+        assert bool(((got.double() - ref).abs() <= attention_tolerance(c64, table, lengths, q, scale, dtype, ref)).all())
+    got = attention(gpu, dc, table, q, lengths, scale, dtype, max_len=top)
+    right(got, lengths)
+    out = torch.zeros_like(got)
+    b = [dev(gpu, t) for t in (torch.from_numpy(table), q, out, i32(lengths))]
+    with gpu.Recording() as rec:
+        gpu.attn_kv8(dc.handle, b[0], table.shape[1], b[1], b[2], b[3], len(lengths), top, H, dtype=code(gpu, dtype))
+    rec.replay(3)
+    assert torch.equal(back(gpu, b[2], out), got)
+    other = [0, 1700, 300, 1025, 256, 899]
+    b[3].upload(np.array(other, np.int32))
+    rec.replay(1)
+    right(back(gpu, b[2], out), other)
+    b[2].upload(torch.full_like(out, 3.0).view(torch.uint8).numpy())
+    b[3].upload(np.array(other[:4] + [top + 1, 899], np.int32))
+    rec.replay(1)
+    last = back(gpu, b[2], out)
+    with pytest.raises(gpu.SimpGpuError):
+        gpu.check(gpu.lib().simp_gpu_check_device_status())
+    assert bool((last[4] == 3.0).all())
+    right(torch.where((torch.arange(6) == 4)[:, None, None], torch.zeros_like(last), last), other[:4] + [0, 899])
+    rec.close()
+
+
 def test_what_lies_behind_a_sequence_is_not_read(gpu):
     """Table entries behind the last block are garbage, scales of blocks in no sequence are NaN, max_len is larger than any
     length: no influence, nothing reported."""

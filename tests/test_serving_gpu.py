@@ -147,15 +147,15 @@ g = torch.Generator().manual_seed(0)
 q = torch.randn(50, 2, 64, generator=g)
 out = torch.zeros_like(q)
 b, bo, off = dev(sg, q), dev(sg, out), dev(sg, offsets([50]))
-c = Cache64(4096 // 16, 16, 1, 64)
+c = Cache64(8192 // 16, 16, 1, 64)
 dc = DeviceCache(sg, c)
-table = dev(sg, torch.arange(256, dtype=torch.int32))
+table = dev(sg, torch.arange(512, dtype=torch.int32))
 ln, qq, oo = dev(sg, i32([4000])), dev(sg, q[:1, :1]), dev(sg, q[:1, :1])
 lg, best = dev(sg, torch.zeros(1, 40000)), sg.DeviceBuffer(16)
 codes = []
 with sg.Recording() as rec:
     sg.attn_prompt(b, b, b, bo, off, None, 1, 50, 50, 2, 2, 64)
-    for call in (lambda: sg.attn_kv8(dc.handle, table, 256, qq, oo, ln, 1, 4096, 1), lambda: sg.logits_process(lg, lg, 1, 40000, sg.logits_rules(), argmax=best)):
+    for call in (lambda: sg.attn_kv8(dc.handle, table, 512, qq, oo, ln, 1, 8192, 1), lambda: sg.logits_process(lg, lg, 1, 40000, sg.logits_rules(), argmax=best)):
         try:
             call()
             codes.append(0)
