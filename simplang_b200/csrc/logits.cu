@@ -37,7 +37,7 @@ __device__ __forceinline__ unsigned long long logit_key(float v, int i) {
 // A thread has U 16-byte vectors in flight; a block works on NSUB times LG_THREADS * U * VEC tokens.
 template <typename T, int U, int NSUB>
 __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) {
-  constexpr int VEC = 16 / sizeof(T), SUB = LG_THREADS * U * VEC, SLICE = SUB * NSUB, LISTED = SLICE / 8;
+  constexpr int VEC = 16 / sizeof(T), SUB = LG_THREADS * U * VEC, SLICE = SUB * NSUB, LISTED = NSUB > 1 ? SLICE / 8 : 0;   // short slices: few entries each, and a step less to wait for
   extern __shared__ __align__(16) int lg_smem[];
   __shared__ unsigned long long wbest[LG_THREADS / 32];
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
@@ -120,9 +120,14 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
     if (he > hb) {
       for (int i0 = hb;;) {
 #pragma unroll
-        for (int k = 0; k < E; ++k)
-          if (ids[k] >= 0 && atomicAdd(changed + ids[k], 1) == 0)
+        for (int k = 0; k < E; ++k) {
+          if (ids[k] < 0) continue;
+          const bool first_of = atomicAdd(changed + ids[k], 1) == 0;
+          if (LISTED > 0 && first_of) {
             if (const int at = atomicAdd(n_listed, 1); at < LISTED) listed[at] = uint16_t(ids[k]);
+          }
+          if (LISTED == 0 && !first_of) ids[k] = -1;
+        }
         i0 += E * LG_THREADS;
         if (i0 >= he) break;
         fetch(i0);
@@ -135,7 +140,15 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
       const float f = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
       changed[id] = __float_as_int(__fsub_rn(f, __fadd_rn(__fmul_rn(freq, float(changed[id])), pres)));
     };
-    if (const int n = *n_listed; n > LISTED) {   // too many to list: the first of a token's places in the history works for all
+    if (LISTED == 0 && he - hb <= E * LG_THREADS) {
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if (ids[k] >= 0) {
+          atomicOr(bits + (ids[k] >> 5), 1u << (ids[k] & 31));
+          penalise(ids[k]);
+        }
+      __syncthreads();
+    } else if (const int n = LISTED > 0 ? *n_listed : 1; n > LISTED) {   // too many to list: the first of a token's places in the history works for all
       for (int i = hb + tid; i < he; i += LG_THREADS) {
         int id = __ldg(a.r.tokens + i);
         if (id < first || id >= last) continue;
