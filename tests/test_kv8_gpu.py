@@ -296,6 +296,33 @@ def test_long_cache_is_split_and_joined(gpu, dtype, H, G, dim):
     rec2.close()
 
 
+@pytest.mark.parametrize("factor", [2, 3, 6, 10, 1.5, 1.0078125, 63.5, 254])
+@pytest.mark.parametrize("step", [1.0, 0.3, 3e-38])
+def test_larger_steps_keep_halves_even(gpu, factor, step):
+    """A block that grows by a factor that puts many held integers on halves: q old / new rounded to even, exactly."""
+    bt, dim, held = 64, 32, 45
+    step = np.float32(step)
+    q = ((np.arange(held * dim) * 37) % 255 - 127).reshape(held, 1, dim)
+    q[0, 0, 0] = 127
+    first = (q * step).astype(np.float32)
+    old = np.float32(np.abs(first).max() / np.float32(127.0))
+    assert np.array_equal(np.rint(first.astype(np.float64) / old), q)
+    last = np.zeros((1, 1, dim), np.float32)
+    last[0, 0, 5] = -np.float32(127.0) * np.float32(factor) * step
+    new = np.float32(np.abs(last).max() / np.float32(127.0))
+    want = np.rint(q.astype(np.float64) * np.float64(old) / np.float64(new))
+    kb, vb, ks, vs = (gpu.DeviceBuffer(n) for n in gpu.kv8_bytes(1, bt, 1, dim))
+    cache = gpu.kv8_cache(kb, vb, ks, vs, 1, bt, 1, dim)
+    table, zero = dev(gpu, i32([0])), dev(gpu, i32([0]))
+    for rows_, at in ((first, 0), (last, held)):
+        b = gpu.DeviceBuffer.from_numpy(rows_)
+        gpu.kv8_append(cache, table, 1, b, b, dev(gpu, i32([0, len(rows_)])), dev(gpu, i32([at])), 1, len(rows_))
+    assert ks.to_numpy(np.float32, (1,))[0] == new and vs.to_numpy(np.float32, (1,))[0] == new
+    k = kb.to_numpy(np.int8, (bt, dim))[:held].reshape(held, 1, dim)
+    v = vb.to_numpy(np.int8, (bt // 16, dim, 16)).transpose(0, 2, 1).reshape(bt, dim)[:held].reshape(held, 1, dim)
+    assert np.array_equal(k, want) and np.array_equal(v, want)
+
+
 @pytest.mark.parametrize("dtype,H,G,dim", [("f32", 4, 1, 64), ("bf16", 8, 1, 128), ("f16", 6, 2, 100), ("f32", 12, 12, 33)])
 def test_chunks_joined_in_a_cluster(gpu, dtype, H, G, dim):
     """Up to eight chunks, of which a sequence needs none, one, some or all; the same bits each time, recorded too, for other
