@@ -37,7 +37,7 @@ template <int D>
 struct F3Shape {
   static constexpr int KEYS = 128, ATOM = KEYS * 128;   // bytes of 64 elements of a tile's rows
   static constexpr int PLANE = KEYS * D * 2, STAGE = 3 * PLANE;
-  static constexpr int BARS = 8;
+  static constexpr int BARS = 9;
   static constexpr size_t SMEM = 2 * size_t(STAGE) + BARS * 8 + 16 + 16 * 128 + 24;
   // TMEM columns: S, which the planes of P replace (192: see place_of_p), T (head sizes up to 64: three), three planes of Q
   static constexpr uint32_t T = 192, Q = T + (D == 64 ? 3 * 64 : 128);
@@ -53,7 +53,6 @@ __host__ __device__ constexpr uint32_t place_of_p(int step, int plane) {
 struct F3Args {
   AttnPromptArgs a;
   int tpt;
-  const uint16_t* q;   // planes [3][total_q][H][D]
   const int* any;   // set: some element is not finite; then the bytes of its row and head are set:
   const uint8_t *odd_q, *odd_k, *odd_v;
 };
@@ -67,13 +66,13 @@ __device__ __forceinline__ void tmem_st_1(uint32_t t, uint32_t v) { asm volatile
 
 template <int D>
 __global__ void __launch_bounds__(F3_THREADS, 1)
-    attn_prompt_f32_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const F3Args p) {
+    attn_prompt_f32_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const F3Args p) {
   using Sh = F3Shape<D>;
   constexpr int KEYS = Sh::KEYS, MINE = 32;   // keys of a tile, of a thread
   extern __shared__ __align__(1024) uint8_t f3_raw[];
   const uint32_t base = smem_u32(f3_raw), k_smem = base, v_smem = base + Sh::STAGE, bars = base + 2 * Sh::STAGE;
   auto k_full = [&](int plane) { return bars + 8u * plane; };
-  const uint32_t v_full = bars + 24, s_bar = bars + 32, p_bar = bars + 40, t_bar = bars + 48, q_bar = bars + 56;
+  const uint32_t v_full = bars + 24, s_bar = bars + 32, p_bar = bars + 40, t_bar = bars + 48, q_bar = bars + 56, q_full = bars + 64;
   uint8_t* tail = f3_raw + 2 * Sh::STAGE + Sh::BARS * 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8);
@@ -92,6 +91,7 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
     mbar_init(p_bar, 16);
     mbar_init(t_bar, 1);
     mbar_init(q_bar, 16);
+    mbar_init(q_full, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -155,6 +155,12 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
           for (int i = 0; i < boxes(j); ++i)
             tma_load_3d(dst + s * Sh::PLANE + b * Sh::ATOM + i * (Sh::ATOM / 2), map, full, 64 * b, g, int(s * a.total_k) + k0 + KEYS * j + 64 * i);
       };
+      // Q first, where V(0) will lie; from there the softmax warps take it to TMEM
+      const int rows = p.tpt * a.rep;
+      mbar_arrive_expect_tx(q_full, 3 * (D / 64) * rows * 128);
+      for (int s = 0; s < 3; ++s)
+        for (int b = 0; b < D / 64; ++b)
+          tma_load_3d(v_smem + s * Sh::PLANE + b * Sh::ATOM, &map_q, q_full, 64 * b, g * a.rep, int(s * a.total_q) + q0 + r0);
       for (int j = 0; ok && j < n; ++j) {
         ok = j == 0 || wait_bar(s_bar, (j - 1) & 1, abort_flag, a.status, 71);
         if (!ok) break;
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
           mbar_arrive_expect_tx(k_full(s), boxes(j) * (Sh::PLANE / 2));
           plane(&map_k, k_smem, k_full(s), s, j);
         }
-        ok = j == 0 || wait_bar(t_bar, (j - 1) & 1, abort_flag, a.status, 82);
+        ok = j == 0 ? wait_bar(q_bar, 0, abort_flag, a.status, 83) : wait_bar(t_bar, (j - 1) & 1, abort_flag, a.status, 82);
         if (!ok) break;
         mbar_arrive_expect_tx(v_full, boxes(j) * (Sh::STAGE / 2));
         for (int s = 0; s < 3; ++s) plane(&map_v, v_smem, v_full, s, j);
@@ -244,15 +250,21 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
     const int lim = mine ? sees(token) : 0;
     volatile float* to = part_row + part * 128 + row;
     volatile float* all = part_row + row;
-    // this row's planes of Q, a quarter of a row per thread, to TMEM (rows behind the sequence: zeros)
+    bool ok = n == 0 || wait_bar(q_full, 0, abort_flag, a.status, 84);
+    // this row's planes of Q, a quarter of a row per thread, to TMEM (16-byte pieces of a row lie in the order of the 128-byte swizzle;
+    // read row by row from global memory this took 8000 cycles, a sixth of a block of five steps)
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t(q) * a.total_q + q0 + token) * a.H * D + int64_t(head) * D + (D / 4) * part);
+      const int piece = D / 32 * part;   // of 8 elements
+      const uint8_t* src = f3_raw + Sh::STAGE + q * Sh::PLANE + (piece >> 3) * Sh::ATOM + row * 128;
 #pragma unroll
       for (int h = 0; h < D / 64; ++h) {   // 16 elements
         uint32_t w[8];
-        const uint4 x = mine ? __ldg(src + 2 * h) : make_uint4(0u, 0u, 0u, 0u), y = mine ? __ldg(src + 2 * h + 1) : make_uint4(0u, 0u, 0u, 0u);
-        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint4 x = *reinterpret_cast<const uint4*>(src + ((((piece & 7) + 2 * h + e) ^ (row & 7)) << 4));
+          w[4 * e] = x.x; w[4 * e + 1] = x.y; w[4 * e + 2] = x.z; w[4 * e + 3] = x.w;
+        }
         tmem_st_32x8(tmem + lanes + Sh::Q + uint32_t(D / 2) * q + uint32_t(D / 8) * part + 8u * h, w);
       }
     }
@@ -284,7 +296,6 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
       }
     };
     const f2 c2 = pack_f2(a.scale_log2, a.scale_log2), none = 0;
-    bool ok = true;
     for (int j = 0; j < n; ++j) {
       if (j > 0) {   // while the scores are multiplied
         ok = __all_sync(0xffffffffu, wait_bar(t_bar, (j - 1) & 1, abort_flag, a.status, 79)) && ok;
@@ -377,11 +388,10 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
     }
     *to = l;
     ok = all_of(1 + (warp & 3), 128, ok);
-    if (ok && mine) {
+    if (ok) {
       l = (all[0] + all[128]) + (all[256] + all[384]);
-      float* out = static_cast<float*>(a.out) + int64_t(q0 + token) * a.out_stride + int64_t(head) * a.D + (D / 4) * part;
       const int cols = a.D - (D / 4) * part;
-      if (any)
+      if (any && mine)
 #pragma unroll 1
         for (int key = 0; key < lim; ++key) {
           if (!p.odd_v[int64_t(k0 + key) * a.G + g]) continue;
@@ -390,19 +400,33 @@ __global__ void __launch_bounds__(F3_THREADS, 1)
           for (int i = 0; i < D / 4; ++i)
             if (i < cols && !(fabsf(v[i]) <= 3.402823466e38f)) o[i] += v[i];
         }
-      const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+      // By way of shared memory (K's place: every MMA is done), so that a warp writes whole rows: 16 bytes of 32 rows at a time
+      // took 5000 cycles.  Rows there are 16 bytes apart in their banks.
+      constexpr int PITCH = D + 4;
+      float* rows = reinterpret_cast<float*>(f3_raw);
+      static_assert(128 * PITCH * 4 <= Sh::STAGE, "");
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int i = 0; i < D / 4; i += 4) {
         float r[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = l == 0.0f ? 0.0f : o[i + e] / l;
-        if (vec && i + 4 <= cols) {
-          *reinterpret_cast<float4*>(out + i) = make_float4(r[0], r[1], r[2], r[3]);
+        for (int e = 0; e < 4; ++e) r[e] = l == 0.0f ? 0.0f : o[i + e] * inv;
+        *reinterpret_cast<float4*>(rows + row * PITCH + (D / 4) * part + i) = make_float4(r[0], r[1], r[2], r[3]);
+      }
+      all_of(1 + (warp & 3), 128, true);
+      const bool vec = a.D % 4 == 0 && a.out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+      const int first = 32 * (warp & 3) + 8 * part;
+      int to_token = r0 + first / a.rep, to_head = first % a.rep;
+#pragma unroll 1
+      for (int at = first; at < min(first + 8, p.tpt * a.rep) && to_token < nq; ++at) {
+        float* out = static_cast<float*>(a.out) + int64_t(q0 + to_token) * a.out_stride + int64_t(g * a.rep + to_head) * a.D;
+        const float* from = rows + at * PITCH;
+        if (vec) {
+          if (4 * lane < a.D) *reinterpret_cast<float4*>(out + 4 * lane) = *reinterpret_cast<const float4*>(from + 4 * lane);
         } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (i + e < cols) out[i + e] = r[e];
+          for (int d = lane; d < a.D; d += 32) out[d] = from[d];
         }
+        if (++to_head == a.rep) to_head = 0, ++to_token;
       }
     }
   }
@@ -418,15 +442,15 @@ template <int D>
 static int f3_launch(F3Args p, const uint8_t* q, const uint8_t* k, const uint8_t* v) {
   const AttnPromptArgs& a = p.a;
   p.tpt = 128 / a.rep;
-  p.q = reinterpret_cast<const uint16_t*>(q);
-  CUtensorMap mk, mv;
+  CUtensorMap mq, mk, mv;
+  if (int rc = attn_tensor_map(&mq, true, q, 3 * a.total_q, a.H, D, int64_t(a.H) * D, a.rep, p.tpt)) return rc;
   if (int rc = attn_tensor_map(&mk, true, k, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, 64)) return rc;
   if (int rc = attn_tensor_map(&mv, true, v, 3 * a.total_k, a.G, D, int64_t(a.G) * D, 1, 64)) return rc;
   auto kern = attn_prompt_f32_tc_kernel<D>;
   SIMP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(F3Shape<D>::SMEM)));
   const int64_t units = std::min(a.total_q, a.total_q / p.tpt + a.n_seqs) * a.G;
   SIMP_REQUIRE(units <= INT_MAX, SIMP_ERR_SHAPE, "attn_prompt: too many rows and heads");
-  SIMP_CUDA(launch_kernel(kern, dim3(unsigned(units)), dim3(F3_THREADS), F3Shape<D>::SMEM, ctx().stream, true, mk, mv, p));
+  SIMP_CUDA(launch_kernel(kern, dim3(unsigned(units)), dim3(F3_THREADS), F3Shape<D>::SMEM, ctx().stream, true, mq, mk, mv, p));
   return SIMP_OK;
 }
 
