@@ -458,13 +458,32 @@ __global__ void __launch_bounds__(128 + 256 * TILES, 3 - TILES)
     if (ok && n_x[x] > 0) ok = wait_bar(o_bar(x), 0, abort_flag, a.status, 68);
     *to = l;
     ok = all_of(1 + 4 * x + (warp & 3), 64, ok);
+    // Heads of 128 leave by way of shared memory (the place of this tile's Q, which no MMA reads any more), so that a warp writes
+    // whole rows; 16-byte pieces of a row lie in another order per row, for the banks.  bf16, 32 / 8 heads: 64 prompts of 128
+    // tokens 88 -> 80 us, 8 of 1024 144 -> 138.  Heads of 64, whose threads have 64 bytes in a row: 113 -> 117, so they do not.
+    constexpr bool STAGED = D == 128;
+    if (STAGED && ok && n > 0) ok = all_of(1 + 4 * x + (warp & 3), 64, wait_bar(q_bar, 0, abort_flag, a.status, 69));   // (a tile that sees nothing)
     if (ok) {
       tc_fence_after_sync();
       l += *from;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t(q0 + token) * a.out_stride + int64_t(head) * a.D + (D / 2) * half) * 2;
-      uint32_t odd = 0;
-      for (int e = 0; e < TC_EDGE * 4; ++e) odd |= odd_keys[e];
+      uint8_t* const stage = generic + x * Sh::TILE;
+      auto piece = [&](int r, int c) { return stage + r * (2 * D) + ((c ^ (r & 7)) << 4); };
+      auto row_of = [&](int of, int h) { return static_cast<uint8_t*>(a.out) + (int64_t(q0 + of) * a.out_stride + int64_t(h) * a.D) * 2; };
+      uint8_t* const out = row_of(token, head) + D * half;
+      auto write = [&](uint8_t* at, const uint4& w, int left) {   // `left` elements from here to the head's end
+        if (p.chunk == 8) {
+          if (left > 0) *reinterpret_cast<uint4*>(at) = w;
+        } else if (p.chunk == 4) {
+          if (left > 0) *reinterpret_cast<uint2*>(at) = make_uint2(w.x, w.y);
+          if (left > 4) *reinterpret_cast<uint2*>(at + 8) = make_uint2(w.z, w.w);
+        } else {
+          const uint16_t* e = reinterpret_cast<const uint16_t*>(&w);
+#pragma unroll
+          for (int t = 0; t < 8; ++t)
+            if (t < left) reinterpret_cast<uint16_t*>(at)[t] = e[t];
+        }
+      };
 #pragma unroll
       for (int h = 0; h < D / 64; ++h) {
         uint32_t o[32];
@@ -472,35 +491,23 @@ __global__ void __launch_bounds__(128 + 256 * TILES, 3 - TILES)
           tmem_ld_32x32(o_tmem + 32u * h, o);
           tmem_ld_wait();
         }
-        if (mine) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
+        for (int i = 0; i < 32; ++i) o[i] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint4 w;
-            w.x = pack2<BF16>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
-            w.y = pack2<BF16>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
-            w.z = pack2<BF16>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
-            w.w = pack2<BF16>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
-            const int left = a.D - ((D / 2) * half + 32 * h + 8 * i);   // elements from here to the head's end
-            uint8_t* at = out + 64 * h + 16 * i;
-            if (p.chunk == 8) {
-              if (left > 0) *reinterpret_cast<uint4*>(at) = w;
-            } else if (p.chunk == 4) {
-              if (left > 0) *reinterpret_cast<uint2*>(at) = make_uint2(w.x, w.y);
-              if (left > 4) *reinterpret_cast<uint2*>(at + 8) = make_uint2(w.z, w.w);
-            } else {
-              const uint16_t* e = reinterpret_cast<const uint16_t*>(&w);
-#pragma unroll
-              for (int t = 0; t < 8; ++t)
-                if (t < left) reinterpret_cast<uint16_t*>(at)[t] = e[t];
-            }
-          }
+        for (int i = 0; i < 4; ++i) {
+          uint4 w;
+          w.x = pack2<BF16>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
+          w.y = pack2<BF16>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
+          w.z = pack2<BF16>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
+          w.w = pack2<BF16>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
+          if (STAGED) *reinterpret_cast<uint4*>(piece(row, D / 16 * half + 4 * h + i)) = w;
+          else if (mine) write(out + 64 * h + 16 * i, w, a.D - ((D / 2) * half + 32 * h + 8 * i));
         }
         __syncwarp();
       }
+      uint32_t odd = 0;
+      for (int e = 0; e < TC_EDGE * 4; ++e) odd |= odd_keys[e];
       if (odd && mine) {   // rare: what the edge tiles' V has that is not finite, to the rows that see it
-        uint16_t* o16 = reinterpret_cast<uint16_t*>(out);
         const int cols = min(D / 2, a.D - (D / 2) * half);
 #pragma unroll 1
         for (int key = 128 * edge0; key < lim; ++key) {
@@ -509,9 +516,20 @@ __global__ void __launch_bounds__(128 + 256 * TILES, 3 - TILES)
 #pragma unroll 1
           for (int i = 0; i < cols; ++i)
             if (odd_halves<BF16>(v[i]) & 0xffffu) {
-              const float sum = to_16<BF16>(o16[i]) + to_16<BF16>(v[i]);
-              o16[i] = uint16_t(pack2<BF16>(sum, 0.0f));
+              uint16_t& o16 = reinterpret_cast<uint16_t*>(STAGED ? piece(row, D / 16 * half + (i >> 3)) : out + 16 * (i >> 3))[i & 7];
+              o16 = uint16_t(pack2<BF16>(to_16<BF16>(o16) + to_16<BF16>(v[i]), 0.0f));
             }
+        }
+      }
+      if constexpr (STAGED) {
+        all_of(1 + 4 * x + (warp & 3), 64, true);
+        const int c = lane & 15;
+        const uint32_t share = 65536u / uint32_t(a.rep) + 1u;   // r * share / 65536 is r / rep for r < 128
+#pragma unroll 2
+        for (int i = 0; i < 16; i += 2) {
+          const int r = 32 * (warp & 3) + 16 * half + i + (lane >> 4), rt = int(uint32_t(r) * share >> 16), to_token = r0 + x * p.tpt + rt;
+          if (r < p.tpt * a.rep && to_token < nq)
+            write(row_of(to_token, g * a.rep + r - rt * a.rep) + 16 * c, *reinterpret_cast<const uint4*>(piece(r, c)), a.D - 8 * c);
         }
       }
     }
