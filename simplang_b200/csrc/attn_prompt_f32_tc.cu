@@ -14,7 +14,8 @@
 // MMA of 64 keys, where it gives 128 bytes a cycle).  That leaves no TMEM for a second S, so P replaces S and softmax and
 // MMAs take turns; only T is added up while the next scores are multiplied.  The form before had tiles of 64 keys, whose S
 // and P lay apart, and overlapped the two: an MMA of 64 keys takes no less time than one of 96 (50 cycles, 75 beside the
-// softmax), so it lost more than it won (4 prompts of 2048, 32 heads of 128: 1180 us, now 1020; of 100: 1265, now 985).
+// softmax), so it lost more than it won (4 prompts of 2048, 32 heads of 128: 1180 us, and 1020 in this form; of 100: 1265 and 985).
+// With Q through shared memory and whole rows written these take 930 and 905 us.
 // A step of 128 keys takes 10700 cycles: 4200 S (48 MMAs, 64 cycles each when nothing loads), 2650 softmax (1024 of them
 // exponentials), 3100 T, the rest hand-overs.  Loading V later, when no MMA runs, costs more than it gives (1085 us).
 // Head sizes up to 64 have half the MMAs for S and keep T apart for each plane of V, which lets one MMA multiply a plane of P

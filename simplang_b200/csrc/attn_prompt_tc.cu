@@ -10,7 +10,7 @@
 //   warps 4-11, 12-19  softmax of tile A, of tile B: two threads per row, 64 keys each, which exchange their maxima
 // P (16 bits) overwrites S in place: S_X(j + 1) is issued behind O_X += P_X(j) V(j) by the same thread, whose MMAs run in order.
 // While the tensor cores work on one tile, the other tile's softmax runs: 2 x 128 x 128 x D MACs take 4 D cycles per tile and
-// step, its 16384 exponentials 1024.  Measured for D = 128 (one prompt of 8192, 32 / 8 heads: 543 us, 1012 TFLOP/s, 0.62 of
+// step, its 16384 exponentials 1024.  Measured for D = 128 (one prompt of 8192, 32 / 8 heads: 536 us, 1026 TFLOP/s, 0.63 of
 // the measured rate): both tiles' steps take 3800 cycles, a tile's chain of 1700 softmax, 200 maxima, 100 P, 250 hand-over,
 // 1250 MMAs and 250 hand-over back.  The tensor cores and the exponentials are each busy a little over half of the time; the
 // softmax is held up by its two warps per scheduler issuing in order (exponentials in polynomial form on the FMA pipe cost
@@ -581,7 +581,7 @@ static int tc_launch(TcArgs p) {
   if (int rc = attn_tensor_map(&mk, BF16, p.k, a.total_k, a.G, D, p.kv_stride, 1, 128)) return rc;
   if (int rc = attn_tensor_map(&mv, BF16, p.v, a.total_k, a.G, D, p.kv_stride, 1, 128)) return rc;
   // Short prompts on one tile per block and two blocks per SM.  32/8 heads, us with one / two tiles: D = 64, 64 prompts of 128
-  // tokens 64 / 73, 16 of 512 86 / 88, 4 of 2048 172 / 172; D = 128, 64 of 1 17 / 28, 64 of 128 88 / 97, 32 of 256 101 / 96.
+  // tokens 64 / 76, 16 of 512 87 / 91, 4 of 2048 173 / 168; D = 128, 64 of 1 18 / 31, 64 of 128 82 / 91, 32 of 256 98 / 91.
   const bool brief = a.total_k < (D == 64 ? 2048 : 192) * int64_t(a.n_seqs);
   return brief ? tc_run<BF16, D, 1>(p, mq, mk, mv) : tc_run<BF16, D, 2>(p, mq, mk, mv);
 }
